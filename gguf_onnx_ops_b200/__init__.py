@@ -5,8 +5,10 @@ host-side mirror of the reference's custom-op interface (``ops``)."""
 from . import _lib  # noqa: F401
 from ._lib import LIB_PATH, GgufOpsError, load  # noqa: F401
 from .ops import (  # noqa: F401
-    MoeRouteGGUF, MoeVerify, Nvfp4Gemv, Q4Gemv, Q8Gemv, dequantize, device_status, set_pdl,
+    DraftVerify, KvAttentionWorkspace, KvCache, KvCacheAttention, KvCacheRead, KvCacheWrite, MoeRouteGGUF, MoeVerify,
+    Nvfp4Gemv, Q4Gemv, Q8Gemv, QkNormRope, dequantize, device_status, set_pdl,
 )
 
-__all__ = ["Q8Gemv", "Q4Gemv", "Nvfp4Gemv", "MoeRouteGGUF", "MoeVerify", "dequantize", "load", "LIB_PATH",
+__all__ = ["Q8Gemv", "Q4Gemv", "Nvfp4Gemv", "MoeRouteGGUF", "MoeVerify", "QkNormRope", "KvCache",
+           "KvCacheWrite", "KvCacheRead", "KvCacheAttention", "KvAttentionWorkspace", "DraftVerify", "dequantize", "load", "LIB_PATH",
            "GgufOpsError", "set_pdl", "device_status"]

@@ -51,6 +51,12 @@ SIGNATURES = {
     "gguf_ipc_open": (_I32, [_P, ctypes.POINTER(ctypes.c_void_p)]),
     "gguf_ipc_close": (_I32, [_P]),
     "gguf_dequantize": (_I32, [_I32, _P, _P, _I64, _I64, _P]),
+    "gguf_qk_norm_rope": (_I32, [_P] * 8 + [_I64] * 7 + [_F32, _I32, _P]),
+    "gguf_kv_cache_write": (_I32, [_P] * 6 + [_I64] * 7 + [_P]),
+    "gguf_kv_cache_read": (_I32, [_P] * 5 + [_I64] * 3 + [_P]),
+    "gguf_kv_cache_attention_workspace": (_I32, [_I64] * 5 + [ctypes.POINTER(ctypes.c_int64)] * 2),
+    "gguf_kv_cache_attention": (_I32, [_P] * 9 + [_I64] * 6 + [_F32, _I64, _P]),
+    "gguf_draft_verify": (_I32, [_P] * 8 + [_I64] * 3 + [_P]),
     "gguf_device_status": (_I32, [ctypes.POINTER(ctypes.c_int)]),
     "gguf_set_pdl": (None, [_I32]),
     "gguf_set_fast_paths": (None, [_I32]),
@@ -106,6 +112,14 @@ class GgufPeerReduce(ctypes.Structure):
 
     _fields_ = [("slots", ctypes.c_void_p * 8), ("flags", ctypes.c_void_p * 8), ("state", ctypes.c_void_p),
                 ("world", ctypes.c_int), ("rank", ctypes.c_int), ("r_max", ctypes.c_int64)]
+
+
+class GgufKvCache(ctypes.Structure):
+    """Mirror of GgufKvCache (include/gguf_ops.h)."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("page", ctypes.c_int64), ("head_dim", ctypes.c_int64)]
 
 
 class GgufOpsError(RuntimeError):

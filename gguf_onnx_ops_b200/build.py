@@ -53,12 +53,18 @@ def build(force: bool = False, verbose: bool = False) -> str:
     objs = []
     tmp = os.path.join(LIBDIR, "_obj")
     os.makedirs(tmp, exist_ok=True)
-    cmd = [nvcc(), *ARCH, *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-c", os.path.join(CSRC, "gguf_ops.cu"),
-           "-o", os.path.join(tmp, "gguf_ops.o")]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    subprocess.run(cmd, check=True)
-    objs.append(os.path.join(tmp, "gguf_ops.o"))
+    running = []
+    for unit in ("gguf_ops", "kv_ops"):  # side by side: each takes tens of seconds
+        obj = os.path.join(tmp, unit + ".o")
+        cmd = [nvcc(), *ARCH, *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-c", os.path.join(CSRC, unit + ".cu"),
+               "-o", obj]
+        if verbose:
+            cmd += ["-Xptxas", "-v"]
+        running.append((cmd, subprocess.Popen(cmd)))
+        objs.append(obj)
+    for cmd, p in running:
+        if p.wait() != 0:
+            raise subprocess.CalledProcessError(p.returncode, cmd)
     host_flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-pthread", "-Wall", "-I",
                   os.path.join(ROOT, "include"), "-I", os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
     subprocess.run(["g++", *host_flags, "-c", os.path.join(CSRC, "gguf_file.cc"), "-o", os.path.join(tmp, "gguf_file.o")],

@@ -25,6 +25,8 @@ enum DeviceErrorSite : int {
   kSiteDrainWait = 3,    // producer waited too long for its last copies at exit
   kSitePeerWait = 5,     // a sharded op waited too long for a peer GPU (its row-split words or EP partials)
   kSiteBadStateRow = 6,  // MambaVerify: the device-side state row was outside [0, state_rows) (row 0 used)
+  kSiteBadCachePage = 7, // a KV-cache op met a page number or a position outside the cache (skipped)
+  kSiteBadPosition = 8,  // QkNormRope: a position outside the cos / sin tables (row 0 used)
 };
 
 // A wait on an mbarrier that has not completed after this many nanoseconds is treated as a fault:

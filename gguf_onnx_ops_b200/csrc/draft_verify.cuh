@@ -1,0 +1,179 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//   draft i of a sequence stands iff u_i q_i(x_i) < p_i(x_i)  (no q: u_i < p_i(x_i));  the first that does not ends the run
+//   n = drafts that stand; the next token is drawn from w = max(p_n - q_n, 0) after a rejected draft (no q: p_n without
+//   x_n), from w = p_n after a run that stands whole.
+// The draw inverts the cumulative distribution in whole numbers: W_v = floor(min(w_v, 1) 2^38) (NaN counts as 0),
+// T = sum W_v, target = floor(T floor(u 2^24) / 2^24), token = the lowest v with W_0 + .. + W_v > target.  Sums of whole
+// numbers do not depend on their order, so however the row is cut the token is the same.  Where T is 0 the draw is
+// made from p_n instead, and where that is empty too the token is -1.
+//
+// One cluster of eight CTAs per sequence: each sums its eighth of the row (two fp32 reads a token, nothing kept), the
+// CTAs' totals meet through distributed shared memory, and the one warp whose stretch holds the target reads that stretch
+// again (from the L2) to find the token.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "kv_cache.cuh"
+
+namespace gguf_b200 {
+
+struct DraftArgs {
+  const float *p, *q;      // [B, R + 1, V], [B, R, V] or null
+  const int32_t* draft;    // [B, R]
+  const float *u, *us;     // [B, R], [B]
+  const int32_t* drafts;   // [B] drafts of each sequence, or null: R
+  int32_t *accepted, *tokens;  // [B], [B, R + 1]
+  int R, V;
+};
+
+constexpr int kDraftCtas = 8;
+constexpr int kDraftThreads = 512;
+constexpr int kDraftWarps = kDraftThreads / 32;
+constexpr int kDraftMax = 32;
+
+__device__ __forceinline__ unsigned long long draft_mass(float p, float q) {
+  const float w = fminf(fmaxf(__fsub_rn(p, q), 0.f), 1.f);  // NaN: 0
+  return __float2ull_rz(w * 274877906944.0f);
+}
+
+// kVec values per lane and load (4 needs V % 4 == 0 and 16-byte aligned rows).
+template <int kVec>
+__global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThreads) draft_verify_kernel(const DraftArgs a) {
+  namespace cg = cooperative_groups;
+  __shared__ unsigned long long warp_sum[kDraftWarps], cta_sum[2];
+  pdl_wait();
+  pdl_launch_dependents();
+  auto cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int b = blockIdx.x / kDraftCtas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n_drafts = a.drafts ? max(0, min(a.R, __ldcg(a.drafts + b))) : a.R;
+  const int64_t V = a.V;
+
+  // Every warp decides the run by itself: lane i looks at draft i.
+  bool stands = false;
+  int x = -1;
+  if (lane < n_drafts) {
+    x = __ldcg(a.draft + static_cast<int64_t>(b) * a.R + lane);
+    if (x >= 0 && x < a.V) {
+      const float p = __ldcg(a.p + (static_cast<int64_t>(b) * (a.R + 1) + lane) * V + x);
+      const float q = a.q ? __ldcg(a.q + (static_cast<int64_t>(b) * a.R + lane) * V + x) : 1.f;
+      stands = __fmul_rn(__ldcg(a.u + static_cast<int64_t>(b) * a.R + lane), q) < p;
+    }
+  }
+  const int n = __ffs(~__ballot_sync(0xffffffffu, stands)) - 1 < 0 ? 32 : __ffs(~__ballot_sync(0xffffffffu, stands)) - 1;
+  const bool rejected = n < n_drafts;
+  const int x_n = __shfl_sync(0xffffffffu, x, n & 31);
+  if (rank == 0 && warp == 0) {
+    if (lane == 0) a.accepted[b] = n;
+    for (int i = lane; i <= a.R; i += 32)
+      if (i != n) a.tokens[static_cast<int64_t>(b) * (a.R + 1) + i] = i < n ? x : -1;
+  }
+
+  const float* p = a.p + (static_cast<int64_t>(b) * (a.R + 1) + n) * V;
+  const float* q = rejected && a.q ? a.q + (static_cast<int64_t>(b) * a.R + n) * V : nullptr;
+  const int skip = rejected && !a.q ? x_n : -1;  // the token a certain draft takes out of the row
+  // The row in warp stretches of whole 32 kVec-value steps.
+  const int step = 32 * kVec, steps = (a.V + step - 1) / step, all_warps = kDraftCtas * kDraftWarps;
+  const int w_id = rank * kDraftWarps + warp;
+  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * w_id / all_warps);
+  const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (w_id + 1) / all_warps);
+  auto masses = [&](int s, bool with_q, unsigned long long (&w)[kVec]) {
+    const int v = s * step + lane * kVec;
+    float pv[kVec], qv[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) pv[i] = qv[i] = 0.f;
+    if (v < a.V) {
+      if constexpr (kVec == 4) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + v));
+        pv[0] = f.x, pv[1] = f.y, pv[2] = f.z, pv[3] = f.w;
+        if (q && with_q) {
+          const float4 e = __ldcg(reinterpret_cast<const float4*>(q + v));
+          qv[0] = e.x, qv[1] = e.y, qv[2] = e.z, qv[3] = e.w;
+        }
+      } else {
+        pv[0] = __ldcg(p + v);
+        if (q && with_q) qv[0] = __ldcg(q + v);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) w[i] = with_q && v + i == skip ? 0ull : draft_mass(pv[i], qv[i]);
+  };
+
+  int token = -1;
+  bool mine = false;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {  // pass 1: the residual is empty, draw from p_n
+    const bool with_q = pass == 0;
+    unsigned long long sum = 0;
+#pragma unroll 4
+    for (int s = s0; s < s1; ++s) {
+      unsigned long long w[kVec];
+      masses(s, with_q, w);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) sum += w[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) warp_sum[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      unsigned long long c = 0;
+      for (int w = 0; w < kDraftWarps; ++w) c += warp_sum[w];
+      cta_sum[pass] = c;
+    }
+    cluster.sync();
+    unsigned long long total = 0, before = 0;
+#pragma unroll
+    for (int r = 0; r < kDraftCtas; ++r) {
+      const unsigned long long c = *cluster.map_shared_rank(&cta_sum[pass], r);
+      total += c;
+      if (r < rank) before += c;
+    }
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    if (total == 0) {
+      mine = rank == 0 && warp == 0 && lane == 0;
+      __syncthreads();  // warp_sum is written again
+      continue;
+    }
+    const float uf = __ldcg(a.us + b) * 16777216.0f;
+    const unsigned long long u = static_cast<unsigned long long>(fminf(fmaxf(uf, 0.f), 16777215.0f));
+    const unsigned long long target = (total >> 24) * u + (((total & 0xFFFFFFull) * u) >> 24);
+    mine = false;
+    if (before <= target && target < before + sum) {  // in this warp's stretch
+      unsigned long long run = before;
+      for (int s = s0; s < s1; ++s) {
+        unsigned long long w[kVec], c = 0;
+        masses(s, with_q, w);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) c += w[i];
+        unsigned long long incl = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, run + incl > target);
+        if (hit) {
+          mine = lane == __ffs(hit) - 1;
+          unsigned long long low = run + incl - c;
+          for (int i = 0; i < kVec; ++i) {
+            low += w[i];
+            if (low > target) {
+              token = s * step + lane * kVec + i;
+              break;
+            }
+          }
+          break;
+        }
+        run += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    break;
+  }
+  if (mine) a.tokens[static_cast<int64_t>(b) * (a.R + 1) + n] = token;
+  cluster.sync();  // no CTA leaves while another may still read its sum
+}
+
+}  // namespace gguf_b200

@@ -16,6 +16,7 @@
 #include <string>
 
 #include "../../include/gguf_ops.h"
+#include "host.cuh"
 #include "engine.cuh"
 #include "slice_r1.cuh"
 #include "slice_iq2_i8.cuh"
@@ -797,9 +798,11 @@ bool int_range(int64_t v) { return v > 0 && v < (1ll << 31); }
 
 }  // namespace
 
-// Error channel shared with the host-only translation units (gguf_file.cc).
+// Shared with the other translation units (host.cuh, gguf_file.cc).
 int set_error(int code, const std::string& msg) { return fail(code, msg); }
 void clear_error() { t_last_error.clear(); }
+bool pdl_enabled() { return g_pdl.load() != 0; }
+int device_sms(int* sms) { return current_sms(sms); }
 
 }  // namespace gguf_b200
 
@@ -1637,6 +1640,9 @@ int gguf_device_status(int* device_error_site) {
   if ((e = cudaMemcpyFromSymbol(&site, g_dev_error_site, sizeof(int))) != cudaSuccess) return cuda_fail("status read", e);
   if ((e = cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(int))) != cudaSuccess) return cuda_fail("status clear", e);
   if ((e = cudaMemcpyToSymbol(g_dev_error_site, &zero, sizeof(int))) != cudaSuccess) return cuda_fail("status clear", e);
+  int kv_err = 0, kv_site = 0;
+  if ((e = kv_device_error(&kv_err, &kv_site)) != cudaSuccess) return cuda_fail("status read", e);
+  if (!err && kv_err) err = kv_err, site = kv_site;
   if (device_error_site) *device_error_site = site;
   return err ? GGUF_ERR_DEVICE : GGUF_OK;
 }

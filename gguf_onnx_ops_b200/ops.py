@@ -21,6 +21,16 @@ C ABI of libgguf_onnx_ops.so on the current torch CUDA stream.
     MambaStep / MambaStepGGUF / MambaVerify / MambaVerifyGGUF       -> y, conv_state, ssm_state, xbc, ypre
                                                                    src/bolt_ops.cu:68-378, :1886-1946
 
+The attention side of a decode / verify step has no counterpart in the reference (no attention op there) and follows the
+same conventions:
+
+    QkNormRope(qkv, q_gamma, k_gamma, cos, sin, positions, heads, kv_heads)    -> q, k
+    KvCache(k, v, k_scale, v_scale)                                            the paged 8-bit cache
+    KvCacheWrite(k, v, cache, page_table, lens, new_lens=None)                 in place
+    KvCacheRead(cache, page_table, lens, rows)                                 -> k, v
+    KvCacheAttention(q, cache, page_table, lens, new_lens=None, scale, window) -> out (, lse)
+    DraftVerify(target_probs, draft_probs, draft_tokens, u_accept, u_sample)   -> accepted, tokens
+
 Every weight layout of the GEMVs is implemented: the GGUF ones (``gguf=1`` / ``iq2=3``) and the
 legacy split layouts (``gguf=0``, ``iq2`` in 0..2, through ``gguf_gemv_legacy``).  The lower-level
 ``*_into`` functions write into caller-provided outputs (no allocation), for graph capture and
@@ -28,6 +38,8 @@ benchmarking.
 """
 
 from __future__ import annotations
+
+import ctypes
 
 import torch
 
@@ -470,6 +482,272 @@ def MambaVerifyGGUF(proj, conv_state, ssm_state, conv_w, conv_b, dt_bias, A_neg,
     return _mamba("MambaVerifyGGUF", proj, conv_state, ssm_state, conv_w, conv_b, dt_bias, A_neg, D, norm_w,
                   state_row, gguf=True,
                   **{"head_dim": 64, "d_state": 128, "epsilon": 1e-5, "time_step_min": 0.0, **attrs})
+
+
+# ------------------------------------------------------------------------------------------------
+# Attention: head norms and rotation, the 8-bit KV cache, draft verification
+# ------------------------------------------------------------------------------------------------
+def qk_norm_rope_into(x, q_gamma, k_gamma, cos, sin, positions, q, k, T: int, row_stride: int, heads: int, kv_heads: int,
+                      head_dim: int, rot: int, max_pos: int, eps: float, interleaved: int, stream=None) -> None:
+    check(load().gguf_qk_norm_rope(_ptr(x), _ptr(q_gamma), _ptr(k_gamma), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(q),
+                                   _ptr(k), T, row_stride, heads, kv_heads, head_dim, rot, max_pos, eps, interleaved,
+                                   _stream(stream)))
+
+
+def QkNormRope(qkv: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None, cos: torch.Tensor,
+               sin: torch.Tensor, positions: torch.Tensor, *, heads: int, kv_heads: int, epsilon: float = 1e-6,
+               interleaved: bool = False):
+    """Per-head RMS norm of queries and keys (gamma f32 [head_dim], None: no norm) and rotation by the rows
+    `positions` (int32 [T]) of cos / sin f32 [max_pos, rot / 2], in one pass and one rounding to bf16.
+
+    qkv bf16 [..., (heads + 2 * kv_heads) * head_dim], T rows at one stride (queries, keys, values as one projection leaves
+    them); the first rot values of a head turn as pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved.  Returns
+    (q [..., heads, head_dim], k [..., kv_heads, head_dim]); a position outside the tables uses row 0 and is reported by
+    device_status()."""
+    if not qkv.is_cuda:
+        raise ValueError("QkNormRope: qkv must be a CUDA tensor")
+    if qkv.dtype != torch.bfloat16:
+        raise ValueError(f"QkNormRope: qkv must be {torch.bfloat16}, got {qkv.dtype}")
+    if qkv.dim() != 2 or qkv.stride(1) != 1:  # one row stride for all tokens, values side by side
+        qkv2 = qkv.reshape(-1, qkv.shape[-1]) if qkv.is_contiguous() else None
+        if qkv2 is None:
+            raise ValueError("QkNormRope: qkv must be contiguous, or 2-D with contiguous rows")
+    else:
+        qkv2 = qkv
+    T, width = qkv2.shape
+    if heads < 1 or kv_heads < 1 or width % (heads + 2 * kv_heads) != 0:
+        raise ValueError("QkNormRope: qkv width must be (heads + 2 * kv_heads) * head_dim")
+    D = width // (heads + 2 * kv_heads)
+    _need(cos, "cos", torch.float32, "QkNormRope")
+    _need(sin, "sin", torch.float32, "QkNormRope")
+    _need(positions, "positions", torch.int32, "QkNormRope")
+    if cos.dim() != 2 or cos.shape != sin.shape or positions.numel() != T:
+        raise ValueError("QkNormRope: needs cos and sin [max_pos, rot / 2] and one position per row")
+    for t, n in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+        if t is not None:
+            _need(t, n, torch.float32, "QkNormRope")
+            if t.numel() != D:
+                raise ValueError(f"QkNormRope: {n} size mismatch")
+    lead = qkv.shape[:-1]
+    q = torch.empty(*lead, heads, D, dtype=torch.bfloat16, device=qkv.device)
+    k = torch.empty(*lead, kv_heads, D, dtype=torch.bfloat16, device=qkv.device)
+    qk_norm_rope_into(qkv2, q_gamma, k_gamma, cos, sin, positions, q, k, T, qkv2.stride(0), heads, kv_heads, D,
+                      2 * cos.shape[1], cos.shape[0], epsilon, 1 if interleaved else 0)
+    return q, k
+
+
+class KvCache:
+    """The paged 8-bit cache of one attention layer: int8 codes k, v [pages, kv_heads, page, head_dim] and one f32 scale for
+    each page and head, k_scale, v_scale [pages, kv_heads]; a value is code * scale."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "_c", "_ref")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        for t, n, dt in ((k, "k", torch.int8), (v, "v", torch.int8), (k_scale, "k_scale", torch.float32),
+                         (v_scale, "v_scale", torch.float32)):
+            _need(t, n, dt, "KvCache")
+        if k.dim() != 4 or v.shape != k.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+            raise ValueError("KvCache: needs k, v [pages, kv_heads, page, head_dim] and scales [pages, kv_heads]")
+        if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
+            raise ValueError("KvCache: tensors must be on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.kv_heads, self.page, self.head_dim = k.shape
+        if self.page not in (16, 32, 64, 128, 256):
+            raise ValueError("KvCache: page must be 16, 32, 64, 128 or 256 tokens")
+        if self.head_dim not in (64, 96, 128, 192, 256):
+            raise ValueError("KvCache: head_dim must be 64, 96, 128, 192 or 256")
+        self._c = _lib.GgufKvCache(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), self.pages, self.kv_heads, self.page,
+                                   self.head_dim)
+        self._ref = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page: int, head_dim: int, device) -> "KvCache":
+        """A cache of zeros."""
+        codes = [torch.zeros(pages, kv_heads, page, head_dim, dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros(pages, kv_heads, dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+
+def _kv_batch(op, cache, page_table, lens, new_lens):
+    _need(page_table, "page_table", torch.int32, op)
+    _need(lens, "lens", torch.int32, op)
+    B = lens.shape[0] if lens.dim() == 1 else -1
+    if page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError(f"{op}: needs page_table [B, pages of a sequence] and lens [B]")
+    if new_lens is not None:
+        _need(new_lens, "new_lens", torch.int32, op)
+        if new_lens.shape != lens.shape:
+            raise ValueError(f"{op}: new_lens must have one number per sequence")
+    return B, page_table.shape[1]
+
+
+def _kv_rows(op, name, t, B, heads, D):
+    """The strides of t bf16 [B, R, heads, D] whose [heads, D] block is contiguous."""
+    if not t.is_cuda:
+        raise ValueError(f"{op}: {name} must be a CUDA tensor")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{op}: {name} must be {torch.bfloat16}, got {t.dtype}")
+    if t.dim() != 4 or t.shape[0] != B or (heads and t.shape[2] != heads) or t.shape[3] != D:
+        raise ValueError(f"{op}: {name} must be [B, rows, {heads or 'heads'}, {D}]")
+    st = t.stride()
+    if st[3] != 1 or (st[2] != D and t.shape[2] != 1):
+        raise ValueError(f"{op}: the heads of a row of {name} must be contiguous")
+    return st[0], st[1]
+
+
+def kv_cache_write_into(cache: KvCache, k, v, page_table, lens, new_lens, B: int, R: int, cols: int, k_strides, v_strides,
+                        stream=None) -> None:
+    check(load().gguf_kv_cache_write(cache._ref, _ptr(k), _ptr(v), _ptr(page_table), _ptr(lens), _ptr(new_lens), B, R, cols,
+                                     *k_strides, *v_strides, _stream(stream)))
+
+
+def KvCacheWrite(k: torch.Tensor, v: torch.Tensor, cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor,
+                 new_lens: torch.Tensor | None = None) -> None:
+    """Quantises k, v bf16 [B, R, kv_heads, head_dim] (any strides of the first two dimensions) into the cache, in
+    place, at positions lens[b] - n .. lens[b] - 1 of every sequence (n = new_lens[b], default R).
+
+    For each touched page and head, with a = max |x| of the call's tokens there: s' = max(s, a / 127), s = 0 if the call
+    begins the page; code = rint(x * (1 / s')); the page's older codes become rint(code * (s / s')).  A value that is not
+    finite makes the scale NaN.  A shorter lens later (a rollback) needs no call; the scale stays."""
+    B, cols = _kv_batch("KvCacheWrite", cache, page_table, lens, new_lens)
+    ks = _kv_rows("KvCacheWrite", "k", k, B, cache.kv_heads, cache.head_dim)
+    vs = _kv_rows("KvCacheWrite", "v", v, B, cache.kv_heads, cache.head_dim)
+    if v.shape != k.shape:
+        raise ValueError("KvCacheWrite: k and v must have the same shape")
+    kv_cache_write_into(cache, k, v, page_table, lens, new_lens, B, k.shape[1], cols, ks, vs)
+
+
+def kv_cache_read_into(cache: KvCache, page_table, lens, k, v, B: int, rows: int, cols: int, stream=None) -> None:
+    check(load().gguf_kv_cache_read(cache._ref, _ptr(page_table), _ptr(lens), _ptr(k), _ptr(v), B, rows, cols,
+                                    _stream(stream)))
+
+
+def KvCacheRead(cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor, *, rows: int):
+    """The last `rows` tokens of every sequence as bf16: (k, v) [B, rows, kv_heads, head_dim]; row i is position
+    lens[b] - rows + i, zeros where that is negative."""
+    B, cols = _kv_batch("KvCacheRead", cache, page_table, lens, None)
+    if rows < 0:
+        raise ValueError("KvCacheRead: rows must be >= 0")
+    k = torch.empty(B, rows, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.k.device)
+    v = torch.empty_like(k)
+    kv_cache_read_into(cache, page_table, lens, k, v, B, rows, cols)
+    return k, v
+
+
+class KvAttentionWorkspace:
+    """Scratch of KvCacheAttention calls that do not overlap: partial results, and counters that are zero between calls.
+    Grows to the largest call it has served."""
+
+    __slots__ = ("device", "scratch", "counters", "_sizes", "_captured")
+
+    def __init__(self, device, _captured: bool = False):
+        self.device, self._captured = device, _captured
+        self.scratch = self.counters = None
+        self._sizes = {}
+
+    def fit(self, B: int, R: int, heads: int, kv_heads: int, head_dim: int) -> "KvAttentionWorkspace":
+        key = (B, R, heads, kv_heads, head_dim)
+        if key not in self._sizes:
+            if not self._captured and torch.cuda.is_current_stream_capturing():  # its clearing would only be recorded
+                raise ValueError("KvCacheAttention: call fit() of a workspace before it is used in a capture")
+            nbytes, n = ctypes.c_int64(0), ctypes.c_int64(0)
+            check(load().gguf_kv_cache_attention_workspace(*key, ctypes.byref(nbytes), ctypes.byref(n)))
+            if self.scratch is None or self.scratch.numel() < nbytes.value:
+                self.scratch = torch.empty(nbytes.value, dtype=torch.uint8, device=self.device)
+            if self.counters is None or self.counters.numel() < n.value:
+                self.counters = torch.zeros(max(n.value, 1024), dtype=torch.int32, device=self.device)
+            self._sizes[key] = True
+        return self
+
+
+_kv_workspaces: dict = {}
+
+
+def _kv_workspace(device, stream) -> KvAttentionWorkspace:
+    """The workspace kept for calls on this stream.  A call that is being captured gets one of its own, which the
+    graph clears and uses at every replay."""
+    if torch.cuda.is_current_stream_capturing():
+        return KvAttentionWorkspace(device, _captured=True)
+    key = (device, stream)
+    ws = _kv_workspaces.get(key)
+    if ws is None:
+        ws = _kv_workspaces[key] = KvAttentionWorkspace(device)
+    return ws
+
+
+def kv_cache_attention_into(cache: KvCache, q, page_table, lens, new_lens, out, lse, workspace: KvAttentionWorkspace,
+                            B: int, R: int, heads: int, cols: int, q_strides, scale: float, window: int,
+                            stream=None) -> None:
+    check(load().gguf_kv_cache_attention(cache._ref, _ptr(q), _ptr(page_table), _ptr(lens), _ptr(new_lens), _ptr(out),
+                                         _ptr(lse), _ptr(workspace.scratch), _ptr(workspace.counters), B, R, heads, cols,
+                                         *q_strides, scale, window, _stream(stream)))
+
+
+def KvCacheAttention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor,
+                     new_lens: torch.Tensor | None = None, *, scale: float | None = None, window: int = 0,
+                     return_lse: bool = False, workspace: KvAttentionWorkspace | None = None):
+    """Causal attention of the R newest tokens of every sequence over the cache: q bf16 [B, R, heads, head_dim] -> out of
+    the same shape (and the log-sum-exp f32 [B, R, heads]).  Head h reads kv head h // (heads // kv_heads).
+
+    lens[b] counts the new tokens; row r < n (n = new_lens[b], default R) sits at position lens[b] - n + r and sees itself and
+    what is before it, or the last `window` positions of that.  Rows from n on give 0 (lse -inf).  scale defaults to
+    head_dim ** -0.5.  One workspace is kept per device and stream; pass one to calls that share a stream with a
+    captured graph's replay on another."""
+    op = "KvCacheAttention"
+    B, cols = _kv_batch(op, cache, page_table, lens, new_lens)
+    strides = _kv_rows(op, "q", q, B, 0, cache.head_dim)
+    R, heads = q.shape[1], q.shape[2]
+    if heads == 0 or heads % cache.kv_heads != 0:
+        raise ValueError(f"{op}: heads must be a multiple of kv heads")
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty(B, R, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    stream = torch.cuda.current_stream()
+    ws = workspace if workspace is not None else _kv_workspace(q.device, stream.cuda_stream)
+    ws.fit(B, R, heads, cache.kv_heads, cache.head_dim)
+    kv_cache_attention_into(cache, q, page_table, lens, new_lens, out, lse, ws, B, R, heads, cols, strides,
+                            cache.head_dim ** -0.5 if scale is None else scale, window, stream)
+    return (out, lse) if return_lse else out
+
+
+def draft_verify_into(target, draft_probs, draft, u_accept, u_sample, drafts, accepted, tokens, B: int, R: int, V: int,
+                      stream=None) -> None:
+    check(load().gguf_draft_verify(_ptr(target), _ptr(draft_probs), _ptr(draft), _ptr(u_accept), _ptr(u_sample),
+                                   _ptr(drafts), _ptr(accepted), _ptr(tokens), B, R, V, _stream(stream)))
+
+
+def DraftVerify(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, draft_tokens: torch.Tensor,
+                u_accept: torch.Tensor, u_sample: torch.Tensor, drafts: torch.Tensor | None = None):
+    """Which drafted tokens stand against the target's probabilities, and the token after them.
+
+    target_probs f32 [B, R + 1, V]; draft_probs f32 [B, R, V], or None for a drafter that was certain; draft_tokens int32
+    [B, R]; u_accept f32 [B, R] and u_sample f32 [B] in [0, 1); drafts int32 [B]: drafts of each sequence (default R).
+    Draft i stands iff u_accept * draft_probs(x_i) < target_probs(x_i); the next token is drawn from
+    max(target - draft, 0) after a rejected draft, else from the target's row (include/gguf_ops.h says how, in whole
+    numbers).  Returns (accepted int32 [B], tokens int32 [B, R + 1]: the drafts that stand, the next token, -1 after it);
+    accepted[b] is the state_row of the sequence's next MambaVerify."""
+    op = "DraftVerify"
+    _need(target_probs, "target_probs", torch.float32, op)
+    _need(draft_tokens, "draft_tokens", torch.int32, op)
+    _need(u_accept, "u_accept", torch.float32, op)
+    _need(u_sample, "u_sample", torch.float32, op)
+    if draft_tokens.dim() != 2 or target_probs.dim() != 3:
+        raise ValueError(f"{op}: needs target_probs [B, R + 1, V] and draft_tokens [B, R]")
+    B, R = draft_tokens.shape
+    V = target_probs.shape[2]
+    if target_probs.shape[:2] != (B, R + 1) or u_accept.shape != draft_tokens.shape or u_sample.shape != (B,):
+        raise ValueError(f"{op}: needs target_probs [B, R + 1, V], u_accept [B, R] and u_sample [B]")
+    if draft_probs is not None:
+        _need(draft_probs, "draft_probs", torch.float32, op)
+        if draft_probs.shape != (B, R, V):
+            raise ValueError(f"{op}: draft_probs must be [B, R, V]")
+    if drafts is not None:
+        _need(drafts, "drafts", torch.int32, op)
+        if drafts.shape != (B,):
+            raise ValueError(f"{op}: drafts must have one number per sequence")
+    accepted = torch.empty(B, dtype=torch.int32, device=draft_tokens.device)
+    tokens = torch.empty(B, R + 1, dtype=torch.int32, device=draft_tokens.device)
+    draft_verify_into(target_probs, draft_probs, draft_tokens, u_accept, u_sample, drafts, accepted, tokens, B, R, V)
+    return accepted, tokens
 
 
 # ------------------------------------------------------------------------------------------------

@@ -282,6 +282,92 @@ GGUF_OPS_API int gguf_ipc_open(const void* handle64, void** dev_ptr);
 GGUF_OPS_API int gguf_ipc_close(void* dev_ptr);
 
 /*
+ * The attention side of a decode / verify step (no counterpart in the reference, which has no attention op).
+ *
+ * QkNormRope: norms of queries and keys for each head, with the position rotation in the same pass.
+ *   x: bf16, T rows of (heads + 2 kv_heads) * head_dim values (queries, keys, values as one projection leaves them),
+ *   row_stride values apart; q bf16 [T, heads, head_dim], k bf16 [T, kv_heads, head_dim] (values are not touched).
+ *   y = x * rsqrt(mean(x^2) + eps) * gamma per head (gamma f32 [head_dim], NULL: no norm), then the first `rot` values
+ *   turn by the angle of the token's row of cos_table / sin_table f32 [max_pos, rot / 2]: pairs (i, i + rot / 2), or
+ *   (2i, 2i + 1) with interleaved = 1.  fp32 throughout, one rounding to bf16.  A position outside [0, max_pos) uses row 0
+ *   and is reported through gguf_device_status.  T = 0 is a no-op.
+ * Contract: head_dim % 8 == 0, <= 256; rot % 8 == 0, <= head_dim; x 8-byte aligned, row_stride % 4 == 0.
+ */
+GGUF_OPS_API int gguf_qk_norm_rope(const void* x, const float* gamma_q, const float* gamma_k, const float* cos_table,
+                                   const float* sin_table, const int32_t* positions, void* q, void* k, int64_t T,
+                                   int64_t row_stride, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot,
+                                   int64_t max_pos, float eps, int interleaved, void* stream);
+
+/*
+ * The paged 8-bit KV cache: int8 codes [pages, kv_heads, page, head_dim] for K and for V, and one f32 scale for each page
+ * and head [pages, kv_heads]; a value is code * scale.  table i32 [B, table_cols] names the page of each sequence's i-th
+ * stretch of `page` tokens; lens i32 [B] is each sequence's length, a call's new tokens included (they are its last
+ * n: n = new_lens[b], or R where new_lens is NULL, never more than lens[b]).
+ * Contract: head_dim 64, 96, 128, 192 or 256; page 16, 32, 64, 128 or 256; codes 16-byte aligned.  A page number or a
+ * length outside the cache is skipped and reported through gguf_device_status.
+ */
+typedef struct {
+  void *k, *v;               /* int8 [pages, kv_heads, page, head_dim] */
+  float *k_scale, *v_scale;  /* f32 [pages, kv_heads] */
+  int64_t pages, kv_heads, page, head_dim;
+} GgufKvCache;
+
+/*
+ * KvCacheWrite: quantises k, v (bf16 [B, R, kv_heads, head_dim], the first two strides in values) into the cache at
+ * positions lens[b] - n .. lens[b] - 1.  For each touched page and head, with a = max |x| of the call's tokens there:
+ *   s' = max(s, a / 127), where s = 0 if the call begins the page; below the smallest normal float: 0
+ *   code = rint(x * (1 / s')), and the page's older codes become rint(code * (s / s'))
+ * all in fp32.  Writing tokens again, or others in their place after a rollback of lens, keeps s from shrinking until the
+ * page is begun again.  A value that is not finite makes the scale of its page and head NaN.  Two sequences of one call must
+ * not write to the same page.
+ */
+GGUF_OPS_API int gguf_kv_cache_write(const GgufKvCache* cache, const void* k, const void* v, const int32_t* table,
+                                     const int32_t* lens, const int32_t* new_lens, int64_t B, int64_t R,
+                                     int64_t table_cols, int64_t k_stride_b, int64_t k_stride_r, int64_t v_stride_b,
+                                     int64_t v_stride_r, void* stream);
+
+/*
+ * KvCacheRead: the last `rows` tokens of every sequence as bf16(code * scale), k and v [B, rows, kv_heads, head_dim];
+ * row i is position lens[b] - rows + i, zeros where that is negative.
+ */
+GGUF_OPS_API int gguf_kv_cache_read(const GgufKvCache* cache, const int32_t* table, const int32_t* lens, void* k, void* v,
+                                    int64_t B, int64_t rows, int64_t table_cols, void* stream);
+
+/*
+ * KvCacheAttention: causal attention of R query rows per sequence over the cache, q bf16 [B, R, heads, head_dim] (the first
+ * two strides in values), out bf16 [B, R, heads, head_dim], lse f32 [B, R, heads] (natural log-sum-exp) or NULL.  Head h reads kv head
+ * h / (heads / kv_heads).  Row r < n of sequence b sits at position t = lens[b] - n + r and sees positions
+ * max(0, t - window + 1) .. t (window 0: 0 .. t); its output is sum_j softmax_j(scale q.k_j) v_j.  Rows r >= n give 0 (lse
+ * -inf).  workspace and counters have the sizes that gguf_kv_cache_attention_workspace gives for the current device;
+ * counters must be zero before the first call and are left zero.  Calls that may overlap need workspaces of their own.
+ * Contract: B <= 4096.
+ */
+GGUF_OPS_API int gguf_kv_cache_attention_workspace(int64_t B, int64_t R, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                   int64_t* bytes, int64_t* counters);
+GGUF_OPS_API int gguf_kv_cache_attention(const GgufKvCache* cache, const void* q, const int32_t* table,
+                                         const int32_t* lens, const int32_t* new_lens, void* out, float* lse,
+                                         void* workspace, int32_t* counters, int64_t B, int64_t R, int64_t heads,
+                                         int64_t table_cols, int64_t q_stride_b, int64_t q_stride_r, float scale,
+                                         int64_t window, void* stream);
+
+/*
+ * DraftVerify: which of R drafted tokens stand against the target's probabilities, and the token after them.
+ *   target f32 [B, R + 1, V] (row i: the target's distribution after i drafts), draft_probs f32 [B, R, V] (the
+ *   distribution draft i was drawn from) or NULL (the drafter was certain of its token), draft i32 [B, R],
+ *   u_accept f32 [B, R] and u_sample f32 [B] in [0, 1), drafts i32 [B] (drafts of each sequence) or NULL: R.
+ *   Draft i stands iff u_accept_i * draft_probs_i(x_i) < target_i(x_i); accepted[b] = drafts before the first that does not.
+ *   The next token is drawn from max(target - draft_probs, 0) of the rejected draft's rows, or from target's row after the
+ *   last draft: with W_v = floor(min(w_v, 1) * 2^38) and T = sum W, the lowest v with W_0 + .. + W_v >
+ *   floor(T * floor(u_sample * 2^24) / 2^24).  An empty residual is replaced by target's row; an empty row gives -1.
+ *   accepted i32 [B]; tokens i32 [B, R + 1] = the drafts that stand, the next token, then -1.
+ * accepted[b] is the state_row that the next gguf_mamba_step (Verify) of the sequence starts from.
+ * Contract: 1 <= R <= 32, V <= 2^24.
+ */
+GGUF_OPS_API int gguf_draft_verify(const float* target, const float* draft_probs, const int32_t* draft,
+                                   const float* u_accept, const float* u_sample, const int32_t* drafts,
+                                   int32_t* accepted, int32_t* tokens, int64_t B, int64_t R, int64_t V, void* stream);
+
+/*
  * Dequantise raw GGUF rows to f32 with the same device decoders the GEMVs use (debug / parity
  * entry point; no counterpart op in the reference).  type = GGUF_TYPE_*; w [rows, row_bytes(K)];
  * out f32 [rows, K].  Results are bit-identical to gguf-py 0.19.0 dequantize.
