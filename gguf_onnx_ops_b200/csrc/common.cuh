@@ -27,6 +27,7 @@ enum DeviceErrorSite : int {
   kSiteBadStateRow = 6,  // MambaVerify: the device-side state row was outside [0, state_rows) (row 0 used)
   kSiteBadCachePage = 7, // a KV-cache op met a page number or a position outside the cache (skipped)
   kSiteBadPosition = 8,  // QkNormRope: a position outside the cos / sin tables (row 0 used)
+  kSiteTileWait = 9,     // KvCacheAttention's warps waited too long for one another
 };
 
 // A wait on an mbarrier that has not completed after this many nanoseconds is treated as a fault:

@@ -48,18 +48,18 @@ __global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThrea
   auto cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   const int b = blockIdx.x / kDraftCtas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n_drafts = a.drafts ? max(0, min(a.R, __ldcg(a.drafts + b))) : a.R;
+  const int n_drafts = a.drafts ? max(0, min(a.R, ld_cg(a.drafts + b))) : a.R;
   const int64_t V = a.V;
 
   // Every warp decides the run by itself: lane i looks at draft i.
   bool stands = false;
   int x = -1;
   if (lane < n_drafts) {
-    x = __ldcg(a.draft + static_cast<int64_t>(b) * a.R + lane);
+    x = ld_cg(a.draft + static_cast<int64_t>(b) * a.R + lane);
     if (x >= 0 && x < a.V) {
-      const float p = __ldcg(a.p + (static_cast<int64_t>(b) * (a.R + 1) + lane) * V + x);
-      const float q = a.q ? __ldcg(a.q + (static_cast<int64_t>(b) * a.R + lane) * V + x) : 1.f;
-      stands = __fmul_rn(__ldcg(a.u + static_cast<int64_t>(b) * a.R + lane), q) < p;
+      const float p = ld_cg(a.p + (static_cast<int64_t>(b) * (a.R + 1) + lane) * V + x);
+      const float q = a.q ? ld_cg(a.q + (static_cast<int64_t>(b) * a.R + lane) * V + x) : 1.f;
+      stands = __fmul_rn(ld_cg(a.u + static_cast<int64_t>(b) * a.R + lane), q) < p;
     }
   }
   const int n = __ffs(~__ballot_sync(0xffffffffu, stands)) - 1 < 0 ? 32 : __ffs(~__ballot_sync(0xffffffffu, stands)) - 1;
@@ -86,15 +86,15 @@ __global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThrea
     for (int i = 0; i < kVec; ++i) pv[i] = qv[i] = 0.f;
     if (v < a.V) {
       if constexpr (kVec == 4) {
-        const float4 f = __ldcg(reinterpret_cast<const float4*>(p + v));
+        const float4 f = ld_cg(reinterpret_cast<const float4*>(p + v));
         pv[0] = f.x, pv[1] = f.y, pv[2] = f.z, pv[3] = f.w;
         if (q && with_q) {
-          const float4 e = __ldcg(reinterpret_cast<const float4*>(q + v));
+          const float4 e = ld_cg(reinterpret_cast<const float4*>(q + v));
           qv[0] = e.x, qv[1] = e.y, qv[2] = e.z, qv[3] = e.w;
         }
       } else {
-        pv[0] = __ldcg(p + v);
-        if (q && with_q) qv[0] = __ldcg(q + v);
+        pv[0] = ld_cg(p + v);
+        if (q && with_q) qv[0] = ld_cg(q + v);
       }
     }
 #pragma unroll
@@ -137,7 +137,7 @@ __global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThrea
       __syncthreads();  // warp_sum is written again
       continue;
     }
-    const float uf = __ldcg(a.us + b) * 16777216.0f;
+    const float uf = ld_cg(a.us + b) * 16777216.0f;
     const unsigned long long u = static_cast<unsigned long long>(fminf(fmaxf(uf, 0.f), 16777215.0f));
     const unsigned long long target = (total >> 24) * u + (((total & 0xFFFFFFull) * u) >> 24);
     mine = false;

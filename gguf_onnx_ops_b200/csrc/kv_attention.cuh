@@ -86,22 +86,30 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Predicated loads that leave their registers alone where `on` is false.  Prefetches for the next turn of a loop are written
+// with them: behind a branch the compiler merges the two values with moves, which wait for the load.
+__device__ __forceinline__ void ld_if(uint32_t& w, const void* p, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p ld.global.cg.u32 %0, [%1];\n}\n" : "+r"(w) : "l"(p), "r"(on ? 1u : 0u) : "memory");
+}
 // kBytes consecutive bytes (4, 8 or 16 at a time) of a cache page into words; read once, kept out of L1.
 template <int kBytes>
-__device__ __forceinline__ void load_codes(uint32_t* w, const int8_t* p) {
+__device__ __forceinline__ void load_codes_if(uint32_t* w, const int8_t* p, bool on) {
+  const uint32_t c = on ? 1u : 0u;
   if constexpr (kBytes % 16 == 0) {
 #pragma unroll
     for (int i = 0; i < kBytes / 16; ++i)
-      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "l"(p + 16 * i));
+      asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n @p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n}\n"
+                   : "+r"(w[4 * i]), "+r"(w[4 * i + 1]), "+r"(w[4 * i + 2]), "+r"(w[4 * i + 3]) : "l"(p + 16 * i), "r"(c) : "memory");
   } else if constexpr (kBytes % 8 == 0) {
 #pragma unroll
     for (int i = 0; i < kBytes / 8; ++i)
-      asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[2 * i]), "=r"(w[2 * i + 1]) : "l"(p + 8 * i));
+      asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %3, 0;\n @p ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n}\n"
+                   : "+r"(w[2 * i]), "+r"(w[2 * i + 1]) : "l"(p + 8 * i), "r"(c) : "memory");
   } else {
 #pragma unroll
     for (int i = 0; i < kBytes / 4; ++i)
-      asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[i]) : "l"(p + 4 * i));
+      asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p ld.global.L1::no_allocate.u32 %0, [%1];\n}\n"
+                   : "+r"(w[i]) : "l"(p + 4 * i), "r"(c) : "memory");
   }
 }
 
@@ -111,13 +119,13 @@ struct KvSpan {
 };
 __device__ __forceinline__ KvSpan kv_span(const KvAttnArgs& a, int b) {
   KvSpan s;
-  s.len = max(0, __ldcg(a.lens + b));
+  s.len = max(0, ld_cg(a.lens + b));
   const int cap = a.c.table_cols << a.c.log2_page;
   if (s.len > cap) {
     record_device_error(kSiteBadCachePage);
     s.len = cap;
   }
-  s.n = max(0, min(a.news ? __ldcg(a.news + b) : a.R, min(a.R, s.len)));
+  s.n = max(0, min(a.news ? ld_cg(a.news + b) : a.R, min(a.R, s.len)));
   s.lo = a.window > 0 ? max(0, s.len - s.n + 1 - a.window) : 0;
   s.t0 = s.lo / kKvTile;
   s.t1 = s.n > 0 ? (s.len + kKvTile - 1) / kKvTile : s.t0;
@@ -213,7 +221,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         w[i] = make_uint2(0, 0);
-        if (on && (lane + 32 * i) * 4 < kD) w[i] = ldcg64(qr + (lane + 32 * i) * 4);
+        if (on && (lane + 32 * i) * 4 < kD) w[i] = ld_cg64(qr + (lane + 32 * i) * 4);
         m = abs_max_bf16x2(abs_max_bf16x2(m, w[i].x), w[i].y);
       }
       m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
@@ -257,37 +265,37 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
     all_lo = __reduce_max_sync(0xffffffffu, all_lo);
     all_hi = __reduce_min_sync(0xffffffffu, all_hi);
 
-    uint32_t kw[2][P::kSteps], vw[4][kD / 32];
-    float ks = 0.f, vs = 0.f;
+    uint32_t kw[2][P::kSteps] = {}, vw[4][kD / 32] = {};
+    uint32_t ks = 0, vs = 0;  // bits of the tile's scales
     const int stop = min(sp.t0 + tb, sp.t1);
     int tile = sp.t0 + ta + warp;
     const int lg = a.c.log2_page, in_page = (1 << lg) - 1;
-    auto page_of = [&](int tl) { return static_cast<int64_t>(max(static_cast<int64_t>(0), kv_page(a.c, b, (tl * kKvTile) >> lg))); };
+    const int32_t* table = a.c.table + static_cast<int64_t>(b) * a.c.table_cols;  // (positions below len lie in it)
+    uint32_t entry = 0, entry_next = 0;  // pages of `tile` and of this warp's next tile
+    auto page_of = [&](uint32_t e) { return static_cast<int64_t>(kv_page_ok(a.c, static_cast<int>(e)) ? e : 0); };
     auto row0 = [&](int64_t page, int tl) {
       return ((((page * a.c.kv_heads + h) << lg) + ((tl * kKvTile) & in_page))) * kD;
     };
-    auto load_k = [&](int64_t page, int tl) {
+    auto load_k = [&](int64_t page, int tl, bool on) {
       const int8_t* p = a.k + row0(page, tl) + t * P::kKPiece;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int j = 0; j < kD / (4 * P::kKPiece); ++j)
-          load_codes<P::kKPiece>(&kw[r][j * (P::kKPiece / 4)], p + (g + 8 * r) * kD + j * 4 * P::kKPiece);
+          load_codes_if<P::kKPiece>(&kw[r][j * (P::kKPiece / 4)], p + (g + 8 * r) * kD + j * 4 * P::kKPiece, on);
+      ld_if(ks, a.ks + page * a.c.kv_heads + h, on);
+      ld_if(vs, a.vs + page * a.c.kv_heads + h, on);
     };
-    auto load_v = [&](int64_t page, int tl) {
+    auto load_v = [&](int64_t page, int tl, bool on) {
       const int8_t* p = a.v + row0(page, tl) + g * (kD / 8);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) load_codes<kD / 8>(vw[r], p + (2 * t + (r & 1) + 8 * (r >> 1)) * kD);
+      for (int r = 0; r < 4; ++r) load_codes_if<kD / 8>(vw[r], p + (2 * t + (r & 1) + 8 * (r >> 1)) * kD, on);
     };
-    int64_t page = 0;
-    if (tile < stop) {
-      page = page_of(tile);
-      load_k(page, tile);
-      load_v(page, tile);
-      ks = __ldcg(a.ks + page * a.c.kv_heads + h);
-      vs = __ldcg(a.vs + page * a.c.kv_heads + h);
-    }
-    int64_t page_next = tile + kKvWarps < stop ? page_of(tile + kKvWarps) : 0;
+    ld_if(entry, table + ((tile * kKvTile) >> lg), tile < stop);
+    ld_if(entry_next, table + (((tile + kKvWarps) * kKvTile) >> lg), tile + kKvWarps < stop);
+    int64_t page = page_of(entry);
+    load_k(page, tile, tile < stop);
+    load_v(page, tile, tile < stop);
 
     while (tile < stop) {
       const int next = tile + kKvWarps;
@@ -304,14 +312,12 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
           mma_f16_16816(s[nt], a0, a1, a2, a3, q2.x, q2.y);
         }
       }
-      const float ks_now = ks, vs_now = vs == 0.f ? 1.f : vs;
-      if (next < stop) {
-        load_k(page_next, next);
-        ks = __ldcg(a.ks + page_next * a.c.kv_heads + h);
-        vs = __ldcg(a.vs + page_next * a.c.kv_heads + h);
-      }
-      const int64_t page_now = page_next;
-      if (next + kKvWarps < stop) page_next = page_of(next + kKvWarps);
+      const float ks_now = __uint_as_float(ks), vs_now = vs << 1 == 0 ? 1.f : __uint_as_float(vs);
+      const bool more = next < stop;
+      page = page_of(entry_next);  // (read a tile ahead; page 0 where there is no next tile)
+      load_k(page, next, more);
+      entry_next = more ? entry_next : 0;
+      ld_if(entry_next, table + (((next + kKvWarps) * kKvTile) >> lg), next + kKvWarps < stop);
 
       const float lv = lg2(vs_now), inv_v = __fdividef(1.0f, vs_now);
       const int p0 = tile * kKvTile;
@@ -367,7 +373,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
           for (int nt = 0; nt < kNT; ++nt) mma_f16_16816(o[nt][2 * j + k], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
         }
       }
-      if (next < stop) load_v(page_now, next);
+      load_v(page, next, more);
       tile = next;
     }
 
@@ -448,14 +454,14 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
           float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
           for (int p = 0; p < pieces; ++p) {
             const int64_t sl = 2 * (c_first + p) + (p == 0 ? 1 : 0);
-            mx[0] = fmaxf(mx[0], __ldcg(a.ml + sl * P::kRows + n).x);
-            mx[1] = fmaxf(mx[1], __ldcg(a.ml + sl * P::kRows + n + 1).x);
+            mx[0] = fmaxf(mx[0], ld_cg(a.ml + sl * P::kRows + n).x);
+            mx[1] = fmaxf(mx[1], ld_cg(a.ml + sl * P::kRows + n + 1).x);
           }
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
           for (int p = 0; p < pieces; ++p) {
             const int64_t sl = 2 * (c_first + p) + (p == 0 ? 1 : 0);
-            const float2 u0 = __ldcg(a.ml + sl * P::kRows + n), u1 = __ldcg(a.ml + sl * P::kRows + n + 1);
-            const float4 v = __ldcg(a.part + (sl * P::kFrags + f) * 32 + lane);
+            const float2 u0 = ld_cg(a.ml + sl * P::kRows + n), u1 = ld_cg(a.ml + sl * P::kRows + n + 1);
+            const float4 v = ld_cg(a.part + (sl * P::kFrags + f) * 32 + lane);
             const float f0 = u0.x == -INFINITY ? 0.f : ex2(u0.x - mx[0]), f1 = u1.x == -INFINITY ? 0.f : ex2(u1.x - mx[1]);
             sum[0] = fmaf(u0.y, f0, sum[0]), sum[1] = fmaf(u1.y, f1, sum[1]);
             acc.x = fmaf(v.x, f0, acc.x), acc.y = fmaf(v.y, f1, acc.y);

@@ -1,0 +1,695 @@
+// Attention of many query rows over the 8-bit paged KV cache: 128-row tiles on tcgen05 (the formulas, the scaling of q
+// and the use of V's page scale are those of kv_attention.cuh; w_j <= 2^15 here too, kept so by a running maximum that moves
+// only when it has grown by more than 2^4, with weights scaled to 2^11).
+//
+// Why.  R * heads / kv_heads rows share the K and V of a kv head.  The streaming kernel converts the codes once per 16
+// rows and multiplies on mma.sync; from 17 rows on that work, not the bytes, is its time (48 rows, 16 sequences of up to 9001
+// tokens: 265 us for 25 us of bytes).  Here a CTA converts each 128-token tile of codes once, to f16 in shared
+// memory, for up to 256 rows, and the products run on the 5th-generation tensor cores.
+//
+// One CTA per SM, seven warp groups; the tokens go by in steps of 64:
+//   warps 0-7, 8-15  softmax of stream 0 and 1: two threads per row, scores and O in tensor memory
+//   warps 16-19, 20-23  K and V codes to f16, stored swizzled for the MMAs: three buffers each; warp 27 the page scales
+//   warp 25          copies codes into a ring of steps (bulk copies, a page each: loads through the L1 stop at what the
+//                    28 KB beside this much shared memory hold, 2 us a tile)
+//   warps 24 and 26  issue the MMAs of a stream: S = q K^T (128 x 64), then O += w V with w (f16) in the columns of its S.  Every stream
+//                    has two S, so that the next scores are there before this step's weights are done
+// A stream is a 128-row tile against every step when a unit has two row tiles (256 rows share the converted codes), or
+// one row tile against every second step when it has one (two accumulators, joined at the end).
+// The line of all units' 128-token tiles is cut into equal slices as in the streaming kernel; a second kernel joins the pieces.
+#pragma once
+
+#include <type_traits>
+
+#include "kv_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace gguf_b200 {
+
+constexpr int kTileSoftmax = 512, kTileConvert = 256, kTileThreads = kTileSoftmax + kTileConvert + 128;
+constexpr int kTileConvertWarp = kTileSoftmax / 32, kTileConvertWarps = kTileConvert / 32, kTileMmaWarp = (kTileSoftmax + kTileConvert) / 32;
+// Registers a thread: the kernel is launched with at least kTileLaunchRegs (checked on the host), 64512 in all; the
+// softmax groups then take 88, the converting ones 40 and the last group 72: 45056 + 10240 + 9216 = 64512.
+constexpr int kTileLaunchRegs = 72, kTileSoftmaxRegs = 88, kTileConvertRegs = 40, kTileOtherRegs = 72;
+static_assert(kTileSoftmax * kTileSoftmaxRegs + kTileConvert * kTileConvertRegs + 128 * kTileOtherRegs <= kTileThreads * kTileLaunchRegs,
+              "the shares must fit what the CTA is launched with");
+constexpr int kTileTokens = 128;          // what the work is cut by
+constexpr int kTileStep = 64;             // tokens of a step
+constexpr int kTileMaxBatch = 2048;       // what the shared memory leaves room for (a larger batch is streamed)
+constexpr int kTileBufs = 3;              // K and V buffers
+constexpr int kTileRows = 128;            // of one stream
+constexpr int kTileUnitRows = 2 * kTileRows;
+constexpr float kTileTop = 11.f, kTileGrow = 4.f;  // weights start at 2^11 and may grow to 2^15
+
+template <int kD>
+struct KvTilePlan {
+  static constexpr int kQTile = kTileRows * kD * 2;      // f16 bytes of a q tile
+  static constexpr int kOperand = kTileStep * kD * 2;    // f16 bytes of a step of K or V
+  static constexpr int kBlock = kTileStep * 128;         // of which each 64 values of a head take this much
+  static constexpr int kPieces = kTileStep * kD / 8 / 128;  // 8-code pieces per converting thread
+  static constexpr int kRaw = kTileStep * kD;            // bytes of a staged step of codes
+  static constexpr int kRing = kD == 128 ? 6 : 12;       // staged steps, K and V in turn: 48 KB
+  static constexpr int kVAt = kTileBufs * kOperand, kQAt = 2 * kVAt, kRingAt = kQAt + 2 * kQTile, kCtrlAt = kRingAt + kRing * kRaw;
+  static constexpr int kCtrl = 4080;                     // scales, barriers, small shared state
+  static constexpr int smem(int B) { return 1024 + kCtrlAt + kCtrl + (B + 1) * 4; }
+  // Tensor memory columns of stream s: its two S (the f16 weights over their S), O.
+  __host__ __device__ static constexpr uint32_t s_at(int s, int buf) { return 128u * s + 64u * buf; }
+  __host__ __device__ static constexpr uint32_t o_at(int s) { return 256u + kD * s; }
+  static_assert(smem(kTileMaxBatch) <= 227 * 1024, "shared memory");
+};
+
+struct KvTileCtrl {
+  alignas(16) float scale_k[8][4], lv[8][4], inv_v[8][4];  // by step % 8 and group of 16 tokens
+  uint64_t k_full[kTileBufs], k_empty[kTileBufs], v_full[kTileBufs], v_empty[kTileBufs], raw_full[12], raw_empty[12];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full[2];  // [stream][item % 2]: an item is a stream's step
+  uint32_t tmem;
+  int scan[28];
+  float2 hand[kTileRows];   // maximum and sum of stream 1, handed to stream 0
+  float swap[2][2][kTileRows];  // [stream][half][row]: what a row's two threads tell each other
+};
+static_assert(sizeof(KvTileCtrl) <= 4080, "control block");
+
+// The token tiles of the 256-row unit rt of a sequence: t0 .. t1 - 1.
+__device__ __forceinline__ void kv_tile_range(const KvAttnArgs& a, const KvSpan& s, int rt, int& t0, int& t1) {
+  const int r0 = rt * kTileUnitRows / a.group;
+  if (r0 >= s.n) {
+    t0 = t1 = 0;
+    return;
+  }
+  const int r1 = min(s.n - 1, ((rt + 1) * kTileUnitRows - 1) / a.group);
+  const int hi = s.len - s.n + r1 + 1;
+  const int lo = a.window > 0 ? max(0, s.len - s.n + r0 + 1 - a.window) : 0;
+  t0 = lo / kTileTokens;
+  t1 = (hi + kTileTokens - 1) / kTileTokens;
+}
+
+struct KvTileUnit {
+  KvSpan sp;
+  int b, h, rt, t0, ta, tb, tiles;  // token tiles t0 + ta .. t0 + tb - 1 of this CTA (tb == ta + 1 with nothing to do: work false)
+  int64_t begin;
+  bool work, two;  // two: two row tiles
+};
+__device__ __forceinline__ KvTileUnit kv_tile_unit(const KvAttnArgs& a, const int* prefix, int64_t at, int64_t end) {
+  KvTileUnit u;
+  int b = 0;
+  for (int hi = a.B; hi - b > 1;) {
+    const int mid = (b + hi) >> 1;
+    if (static_cast<int64_t>(prefix[mid]) * a.c.kv_heads <= at) b = mid; else hi = mid;
+  }
+  u.b = b;
+  u.sp = kv_span(a, b);
+  const int per_head = prefix[b + 1] - prefix[b];
+  const int64_t in_seq = at - static_cast<int64_t>(prefix[b]) * a.c.kv_heads;
+  u.h = static_cast<int>(in_seq / per_head);
+  int rem = static_cast<int>(in_seq % per_head), t1 = 0;
+  for (u.rt = 0;; ++u.rt) {
+    kv_tile_range(a, u.sp, u.rt, u.t0, t1);
+    u.tiles = max(1, t1 - u.t0);
+    if (rem < u.tiles || u.rt + 1 >= a.row_tiles) break;
+    rem -= u.tiles;
+  }
+  u.ta = rem;
+  u.tb = static_cast<int>(min(static_cast<int64_t>(u.tiles), rem + (end - at)));
+  u.begin = at - rem;
+  u.work = t1 > u.t0;
+  u.two = a.R * a.group - u.rt * kTileUnitRows > kTileRows;
+  return u;
+}
+
+// Token tiles of every sequence (all row units of one head), summed: prefix[b] before sequence b; returns the total.
+template <int kThreads>
+__device__ __forceinline__ int kv_tile_prefix(const KvAttnArgs& a, int* prefix, int* scan) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int carry = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    int n = 0;
+    if (b0 + tid < a.B) {
+      const KvSpan s = kv_span(a, b0 + tid);
+      for (int rt = 0; rt < a.row_tiles; ++rt) {
+        int t0, t1;
+        kv_tile_range(a, s, rt, t0, t1);
+        n += max(1, t1 - t0);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += x;
+    }
+    if (lane == 31) scan[warp] = n;
+    __syncthreads();
+    int before = carry;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += scan[w];
+      carry += scan[w];
+    }
+    if (b0 + tid < a.B) prefix[b0 + tid + 1] = before + n;
+    if (b0 + tid == 0) prefix[0] = 0;
+    __syncthreads();
+  }
+  return carry;
+}
+__device__ __forceinline__ int64_t kv_tile_ctas(int64_t total, int grid) {
+  return min(static_cast<int64_t>(grid), (total + 1) / 2);
+}
+// Workspace slot of CTA c's piece of stream s: every CTA cuts at most one unit at its front and one at its end.
+__device__ __forceinline__ int64_t kv_tile_slot(int64_t c, bool begins, int s) { return (2 * c + (begins ? 1 : 0)) * 2 + s; }
+
+// A wait that gives up for good after its first timeout (which is recorded).
+__device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t phase, bool& dead) {
+  if (!dead && !mbar_wait(bar, phase & 1u, kSiteTileWait)) dead = true;
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+template <int kD>
+__global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(const KvAttnArgs a) {
+  using P = KvTilePlan<kD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *k_buf = smem, *v_buf = smem + P::kVAt, *q_buf = smem + P::kQAt, *ring = smem + P::kRingAt;
+  KvTileCtrl* ct = reinterpret_cast<KvTileCtrl*>(smem + P::kCtrlAt);
+  int* prefix = reinterpret_cast<int*>(smem + P::kCtrlAt + P::kCtrl);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (warp == kTileMmaWarp) {
+    tmem_alloc(&ct->tmem, 512);
+    if (lane == 0) {
+      for (int i = 0; i < kTileBufs; ++i) {
+        mbar_init(&ct->k_full[i], kTileConvertWarps / 2 + 1), mbar_init(&ct->v_full[i], kTileConvertWarps / 2);
+        mbar_init(&ct->k_empty[i], 2), mbar_init(&ct->v_empty[i], 2);
+      }
+      for (int i = 0; i < 2; ++i) {
+        for (int j = 0; j < 2; ++j) mbar_init(&ct->s_full[i][j], 1), mbar_init(&ct->p_full[i][j], 2 * kTileRows), mbar_init(&ct->pv_done[i][j], 1);
+        mbar_init(&ct->q_full[i], 2 * kTileRows);
+      }
+      for (int i = 0; i < P::kRing; ++i) mbar_init(&ct->raw_full[i], 1), mbar_init(&ct->raw_empty[i], kTileConvertWarps / 2);
+      fence_mbar_init();
+    }
+    tc_fence_before();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int carry = kv_tile_prefix<kTileThreads>(a, prefix, ct->scan);
+  tc_fence_after();
+  // All 512 columns are this CTA's, so they begin at column 0 (KvTilePlan has their use).
+  const int64_t total = static_cast<int64_t>(carry) * a.c.kv_heads, ctas = kv_tile_ctas(total, gridDim.x);
+  const int64_t from = total * blockIdx.x / max(ctas, static_cast<int64_t>(1));
+  const int64_t end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : from;
+  bool dead = false;
+
+  if (warp >= kTileConvertWarp && warp < kTileMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTileConvertRegs));
+    // ---------------------------------------------------------------- codes to f16
+    // Piece i of a thread: 8 codes of token tok + i * kTokStep, one 16-byte chunk of f16, stored at chunk ^ token % 8 of the
+    // token's 128-byte row (tokens of a thread are alike modulo 8).  Eight lanes read 64 bytes in a row and write eight
+    // different chunks: no bank conflicts on either side.
+    // The first group takes K, the second V.
+    constexpr int kParts = kD / 8, kTokStep = 128 / kParts;
+    const int cw = warp & 3, part = lane % kParts, tok = (cw * 32 + lane) / kParts;
+    const bool is_v = warp >= kTileConvertWarp + 4;
+    const int dst = (part >> 3) * P::kBlock + tok * 128 + (((part & 7) ^ (tok & 7)) << 4);
+    const uint8_t* raw0 = ring + tok * kD + part * 8;
+    uint8_t* buf0 = (is_v ? v_buf : k_buf) + dst;
+    uint64_t *full = is_v ? ct->v_full : ct->k_full, *empty = is_v ? ct->v_empty : ct->k_empty;
+    uint32_t slot = is_v ? 1 : 0, slot_use = 0, buf = 0, use = 0;
+    for (int64_t at = from; at < end;) {
+      const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
+      at += u.tb - u.ta;
+      if (!u.work) continue;
+      for (int left = 2 * (u.tb - u.ta); left > 0; --left) {
+        tile_wait(&ct->raw_full[slot], slot_use, dead);
+        uint2 r[P::kPieces];
+#pragma unroll
+        for (int i = 0; i < P::kPieces; ++i) r[i] = *reinterpret_cast<const uint2*>(raw0 + slot * P::kRaw + i * kTokStep * kD);
+        if (use > 0) tile_wait(empty + buf, use - 1, dead);
+#pragma unroll
+        for (int i = 0; i < P::kPieces; ++i) {
+          const uint32_t x0 = r[i].x ^ 0x80808080u, x1 = r[i].y ^ 0x80808080u;
+          *reinterpret_cast<uint4*>(buf0 + buf * P::kOperand + i * kTokStep * 128) =
+              make_uint4(codes_lo_f16x2(x0), codes_hi_f16x2(x0), codes_lo_f16x2(x1), codes_hi_f16x2(x1));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(full + buf);
+          mbar_arrive(&ct->raw_empty[slot]);
+        }
+        if (++buf == kTileBufs) buf = 0, ++use;
+        if ((slot += 2) >= P::kRing) slot -= P::kRing, ++slot_use;
+      }
+    }
+  } else if (warp >= kTileMmaWarp) {  // (keeps what it was launched with)
+    if (warp == kTileMmaWarp + 1) {
+    // ---------------------------------------------------------------- copies of codes
+    const int lg = a.c.log2_page;
+    const int chunk = min(1 << lg, kTileStep), chunks = kTileStep / chunk;  // tokens a copy, copies a step
+    uint32_t n = 0;  // staged steps
+    for (int64_t at = from; at < end;) {
+      const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
+      at += u.tb - u.ta;
+      if (!u.work) continue;
+      const int st_end = 2 * (u.t0 + u.tb);
+      const int32_t* table = a.c.table + static_cast<int64_t>(u.b) * a.c.table_cols;  // (positions below len lie in it)
+      auto wanted = [&](int st) { return lane < chunks && st < st_end && st * kTileStep + lane * chunk < u.sp.len; };
+      auto entry_of = [&](int st) {
+        uint32_t e = 0;
+        ld_if(e, table + ((st * kTileStep + lane * chunk) >> lg), wanted(st));
+        return e;
+      };
+      auto copy = [&](const int8_t* codes, int st, uint32_t entry, bool copies) {
+        const uint32_t slot = n % P::kRing, bytes = chunk * kD;
+        const int64_t src = (((static_cast<int64_t>(entry) * a.c.kv_heads + u.h) << lg) + (st * kTileStep & ((1 << lg) - 1))) * kD;
+        if (n >= P::kRing) tile_wait(&ct->raw_empty[slot], n / P::kRing - 1, dead);
+        const uint32_t count = __popc(__ballot_sync(0xffffffffu, copies));
+        if (lane == 0) mbar_arrive_expect_tx(&ct->raw_full[slot], count * bytes);
+        __syncwarp();
+        if (copies && !dead) bulk_g2s(ring + slot * P::kRaw + lane * bytes, codes + src, bytes, &ct->raw_full[slot]);
+        ++n;
+      };
+      int st = 2 * (u.t0 + u.ta);
+      uint32_t next = entry_of(st), after = entry_of(st + 1);
+      for (; st < st_end; ++st) {
+        const uint32_t entry = next;
+        next = after;
+        after = entry_of(st + 2);
+        const bool copies = wanted(st) && kv_page_ok(a.c, static_cast<int>(entry));
+        copy(a.k, st, entry, copies);
+        copy(a.v, st, entry, copies);
+      }
+    }
+    bool late = false;  // no copy is in flight when the CTA ends
+    for (uint32_t i = n > P::kRing ? n - P::kRing : 0; i < n; ++i) tile_wait(&ct->raw_full[i % P::kRing], i / P::kRing, late);
+    } else if (warp == kTileMmaWarp + 3) {
+    // ---------------------------------------------------------------- page scales
+    // Of a step's four groups of 16 tokens (pages hold whole groups), read two steps ahead: lanes 0-3 K's, lanes 4-7 V's.
+    // A page outside the cache (the copying warp records it) counts as zeros.  K's buffer counts as filled when they are
+    // there too: the softmax reads them once S is.  (Their slot was last read for the step eight before; the products with
+    // K's buffer that are waited for here were issued after that step's weights had been used.)
+    const int lg = a.c.log2_page;
+    uint32_t steps = 0;
+    for (int64_t at = from; at < end;) {
+      const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
+      at += u.tb - u.ta;
+      if (!u.work) continue;
+      const int st_end = 2 * (u.t0 + u.tb);
+      const int32_t* table = a.c.table + static_cast<int64_t>(u.b) * a.c.table_cols;
+      auto entry_of = [&](int st) {
+        const int pos = st * kTileStep + (lane & 3) * 16;
+        uint32_t e = 0xFFFFFFFFu;
+        ld_if(e, table + (pos >> lg), st < st_end && pos < u.sp.len);
+        return e;
+      };
+      auto scale_of = [&](uint32_t e) {
+        uint32_t w = 0;
+        ld_if(w, (lane < 4 ? a.ks : a.vs) + static_cast<int64_t>(static_cast<int>(e)) * a.c.kv_heads + u.h, lane < 8 && e < a.c.pages);
+        return w;
+      };
+      int st = 2 * (u.t0 + u.ta);
+      uint32_t scale = scale_of(entry_of(st)), entry_next = entry_of(st + 1);
+      for (; st < st_end; ++st, ++steps) {
+        const uint32_t buf = steps % kTileBufs, use = steps / kTileBufs;
+        if (use > 0) tile_wait(&ct->k_empty[buf], use - 1, dead);
+        if (lane < 4) {
+          ct->scale_k[steps & 7][lane] = __uint_as_float(scale);
+        } else if (lane < 8) {
+          const float sv = scale << 1 == 0 ? 1.f : __uint_as_float(scale);
+          ct->lv[steps & 7][lane & 3] = lg2(sv);
+          ct->inv_v[steps & 7][lane & 3] = __fdividef(1.f, sv);
+        }
+        scale = scale_of(entry_next);
+        entry_next = entry_of(st + 2);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ct->k_full[buf]);
+      }
+    }
+    } else if (warp == kTileMmaWarp || warp == kTileMmaWarp + 2) {
+    // ---------------------------------------------------------------- MMA issue, a warp per stream
+    // The whole warp walks the stream's items and one elected lane issues.  What the operands depend on is broadcast, so
+    // that the compiler knows it to be uniform: the MMAs take uniform registers, and moving each operand there costs more
+    // than the products.
+    constexpr uint32_t id_s = tc_idesc_f16(kTileRows, kTileStep, false), id_o = tc_idesc_f16(kTileRows, kD, true);
+    const uint64_t q_desc = smem_desc_sw128(smem_u32(q_buf), 16, 1024), k_desc = smem_desc_sw128(smem_u32(k_buf), 16, 1024);
+    const uint64_t v_desc = smem_desc_sw128(smem_u32(v_buf), P::kBlock, 1024);
+    uint32_t steps = 0, done = 0, units = 0;  // of the units before: steps, items of a stream, units
+    for (int64_t at = from; at < end;) {
+      const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
+      at += u.tb - u.ta;
+      if (!u.work) continue;
+      const int tiles = u.tb - u.ta, items = u.two ? 2 * tiles : tiles;
+      tile_wait(&ct->q_full[0], units, dead);
+      tile_wait(&ct->q_full[1], units, dead);
+      ++units;
+      auto run = [&](auto stream, auto two) {
+        constexpr int s = decltype(stream)::value;
+        constexpr bool both = decltype(two)::value;  // both streams take every step, else each every second
+        auto score = [&](int i, uint32_t buf, uint32_t use) {  // S of item i, K in buffer buf, which is in its use-th use
+          const uint32_t odd = __shfl_sync(0xffffffffu, (done + i) & 1, 0);
+          buf = __shfl_sync(0xffffffffu, buf, 0);
+          tile_wait(&ct->k_full[buf], use, dead);
+          if (i > 1) tile_wait(&ct->pv_done[s][odd], (done + i - 2) >> 1, dead);  // the weights over this S are used (all of
+          tc_fence_after();                                                       // them, at a unit's begin)
+          if (elect_one()) {
+            const uint64_t kd = k_desc + buf * (P::kOperand >> 4);
+#pragma unroll
+            for (int k = 0; k < kD / 16; ++k)
+              tc_mma_ss(P::s_at(s, odd), q_desc + (((both && s == 1 ? P::kQTile : 0) + (k >> 2) * (kTileRows * 128) + (k & 3) * 32) >> 4),
+                        kd + (((k >> 2) * P::kBlock + (k & 3) * 32) >> 4), id_s, k > 0);
+            tc_commit(&ct->s_full[s][odd]);
+            tc_commit(&ct->k_empty[buf]);
+            if (!both) tc_commit(&ct->k_empty[buf]);  // for the other stream
+          }
+          __syncwarp();
+        };
+        auto weigh = [&](int i, uint32_t buf, uint32_t use) {  // O of item i
+          const uint32_t odd = __shfl_sync(0xffffffffu, (done + i) & 1, 0);
+          buf = __shfl_sync(0xffffffffu, buf, 0);
+          tile_wait(&ct->v_full[buf], use, dead);
+          tile_wait(&ct->p_full[s][odd], (done + i) >> 1, dead);
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t vd = v_desc + buf * (P::kOperand >> 4);
+#pragma unroll
+            for (int k = 0; k < kTileStep / 16; ++k)
+              tc_mma_ts(P::o_at(s), P::s_at(s, odd) + k * 8, vd + k * (2048 >> 4), id_o, k > 0 || i > 0);
+            tc_commit(&ct->pv_done[s][odd]);
+            tc_commit(&ct->v_empty[buf]);
+            if (!both) tc_commit(&ct->v_empty[buf]);
+          }
+          __syncwarp();
+        };
+        const uint32_t st0 = steps + (both ? 0 : s);
+        uint32_t buf = st0 % kTileBufs, use = st0 / kTileBufs;
+        score(0, buf, use);
+        for (int i = 0; i < items; ++i) {
+          const uint32_t buf_v = buf, use_v = use;
+          buf += both ? 1 : 2;
+          if (buf >= kTileBufs) buf -= kTileBufs, ++use;
+          if (i + 1 < items) score(i + 1, buf, use);
+          weigh(i, buf_v, use_v);
+        }
+      };
+      const std::integral_constant<int, 0> s0;
+      const std::integral_constant<int, 1> s1;
+      if (warp == kTileMmaWarp) {
+        if (u.two) run(s0, std::true_type{}); else run(s0, std::false_type{});
+      } else {
+        if (u.two) run(s1, std::true_type{}); else run(s1, std::false_type{});
+      }
+      steps += 2 * tiles;
+      done += items;
+    }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTileSoftmaxRegs));
+    // ---------------------------------------------------------------- softmax: two threads per row
+    // Thread `half` of a row has 32 of a step's 64 scores and half of the row's q and O.  Four warps per scheduler: with one
+    // thread per row (two warps), waits and tensor-memory latencies left the exp unit idle for two thirds of the time.
+    const int s = warp >> 3, half = warp >> 2 & 1, row = tid & 127;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    float *mine = &ct->swap[s][half][row], *other = &ct->swap[s][half ^ 1][row];
+    uint32_t steps = 0, done = 0;
+    for (int64_t at = from; at < end;) {
+      const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
+      at += u.tb - u.ta;
+      const int rr = u.rt * kTileUnitRows + (u.two ? s : 0) * kTileRows + row, r = rr / a.group;
+      const bool on = r < u.sp.n, exists = r < a.R;
+      const int64_t out_row = (static_cast<int64_t>(u.b) * a.R + r) * a.heads + u.h * a.group + rr % a.group;
+      if (!u.work) {  // none of the unit's rows sees anything
+        if (exists && (u.two || s == 0)) {
+          uint4* o = reinterpret_cast<uint4*>(a.o + out_row * kD) + half * (kD / 16);
+          for (int i = 0; i < kD / 16; ++i) o[i] = make_uint4(0, 0, 0, 0);
+          if (a.lse && half == 0) a.lse[out_row] = -INFINITY;
+        }
+        continue;
+      }
+      // q: largest value to [2^14, 2^15) by a power of two, a negative softmax scale into its sign.
+      // Tokens that the row sees, from this half's first one of the slice on: first .. last - 1; all of the warp's rows see
+      // all_first .. all_last - 1.
+      const int base = (u.t0 + u.ta) * kTileTokens + half * 32, hi = u.sp.len - u.sp.n + r + 1;
+      const int first = on && a.window > 0 ? max(0, hi - a.window) - base : -base, last = (on ? hi : u.sp.len) - base;
+      const int all_first = __reduce_max_sync(0xffffffffu, first), all_last = __reduce_min_sync(0xffffffffu, last);
+      float qs;
+      {
+        const uint4* qr = reinterpret_cast<const uint4*>(a.q + u.b * a.q_stride_b + r * a.q_stride_r +
+                                                         static_cast<int64_t>(u.h * a.group + rr % a.group) * kD) + half * (kD / 16);
+        uint32_t m = 0;
+        uint4 w[kD / 16];
+#pragma unroll
+        for (int i = 0; i < kD / 16; ++i) w[i] = on ? ld_cg128(qr + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kD / 16; ++i)
+          m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(m, w[i].x), w[i].y), w[i].z), w[i].w);
+        m = max(m & 0xFFFFu, m >> 16);
+        *mine = __uint_as_float(m);
+        bar_sync(2 + s, 2 * kTileRows);
+        m = max(m, __float_as_uint(*other));
+        const int e = m ? min(127, 14 - (static_cast<int>(m >> 7) - 127)) : 0;
+        qs = pow2i(-e) * fabsf(a.scale_log2);
+        if (u.two || s == 0) {
+          const float up = a.scale_log2 < 0.f ? -pow2i(e) : pow2i(e);
+          uint8_t* dst = q_buf + s * P::kQTile + row * 128;
+#pragma unroll
+          for (int i = 0; i < kD / 16; ++i) {
+            const int c = half * (kD / 16) + i;
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (row & 7)) << 4)) =
+                make_uint4(pack_f16x2(bf16_lo(w[i].x) * up, bf16_hi(w[i].x) * up), pack_f16x2(bf16_lo(w[i].y) * up, bf16_hi(w[i].y) * up),
+                           pack_f16x2(bf16_lo(w[i].z) * up, bf16_hi(w[i].z) * up), pack_f16x2(bf16_lo(w[i].w) * up, bf16_hi(w[i].w) * up));
+          }
+          fence_proxy_async_smem();
+        }
+        mbar_arrive(&ct->q_full[s]);
+      }
+      const int tiles = u.tb - u.ta, items = u.two ? 2 * tiles : tiles;
+      float m = -INFINITY, l = 0.f;
+      const uint32_t to = P::o_at(s) + lane_off + half * (kD / 2);
+      for (int i = 0; i < items; ++i) {
+        const uint32_t g = done + i;
+        const int st = u.two ? i : 2 * i + s, sl = (steps + st) & 7, g0 = half * 2;  // the half's first group of 16 tokens
+        const int p0 = st * kTileStep;
+        const uint32_t ts = P::s_at(s, g & 1) + lane_off;
+        const bool whole = p0 >= all_first && p0 + 32 <= all_last;
+        uint32_t bits = 0xFFFFFFFFu;  // bit i: token i of the half is seen
+        if (!whole) {
+          const int f = min(max(first - p0, 0), 32), n = min(max(last - p0, 0), 32);
+          bits = n > f ? (0xFFFFFFFFu >> (32 - n)) & (0xFFFFFFFFu << f) : 0u;
+        }
+        tile_wait(&ct->s_full[s][g & 1], g >> 1, dead);
+        tc_fence_after();
+        uint32_t x[32];
+        tmem_ld32(x, ts + half * 32);
+        const float2 sk = *reinterpret_cast<const float2*>(&ct->scale_k[sl][g0]), lv2 = *reinterpret_cast<const float2*>(&ct->lv[sl][g0]);
+        const float2 iv2 = *reinterpret_cast<const float2*>(&ct->inv_v[sl][g0]);
+        const float cs[2] = {qs * sk.x, qs * sk.y}, lv[2] = {lv2.x, lv2.y}, iv[2] = {iv2.x, iv2.y};
+        tmem_wait_ld(x);
+        float mx = -INFINITY;
+        auto largest = [&](auto cut) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float best = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2)
+              best = fmaxf(best, fmaxf(!cut || bits >> (16 * k + j) & 1 ? __uint_as_float(x[16 * k + j]) : -INFINITY,
+                                       !cut || bits >> (16 * k + j + 1) & 1 ? __uint_as_float(x[16 * k + j + 1]) : -INFINITY));
+            if (!cut || bits >> (16 * k) & 0xFFFFu) mx = fmaxf(mx, fmaf(best, cs[k], lv[k]));
+          }
+        };
+        if (whole) largest(std::false_type{}); else largest(std::true_type{});
+        *mine = mx;
+        bar_sync(2 + s, 2 * kTileRows);
+        mx = fmaxf(mx, *other);
+        if (__any_sync(0xffffffffu, mx > m + kTileGrow)) {  // a row's maximum moves: O and the sum shrink
+          const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : ex2(m - mn);
+          m = mn;
+          l *= f;
+          if (i > 0) {
+            tile_wait(&ct->pv_done[s][(g - 1) & 1], (g - 1) >> 1, dead);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < kD / 32; ++c) {
+              uint32_t y[16];
+              tmem_ld16(y, to + c * 16);
+              tmem_wait_ld(y);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
+              tmem_st16(to + c * 16, y);
+            }
+          }
+        }
+        const float top = m == -INFINITY ? 0.f : m - kTileTop;
+        uint32_t w[16];
+        auto weights = [&](auto cut) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float lift = lv[k] - top;
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              float w0 = ex2(fmaf(__uint_as_float(x[16 * k + j]), cs[k], lift)), w1 = ex2(fmaf(__uint_as_float(x[16 * k + j + 1]), cs[k], lift));
+              if constexpr (cut) {
+                w0 = bits >> (16 * k + j) & 1 ? w0 : 0.f;
+                w1 = bits >> (16 * k + j + 1) & 1 ? w1 : 0.f;
+              }
+              sum[0] += w0, sum[1] += w1;
+              w[k * 8 + j / 2] = pack_f16x2(w0, w1);
+            }
+            if (!cut || bits >> (16 * k) & 0xFFFFu) l = fmaf(sum[0] + sum[1], iv[k], l);  // (a hidden page's scale may be anything)
+          }
+        };
+        if (whole) weights(std::false_type{}); else weights(std::true_type{});
+        tmem_st16(ts + half * 16, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ct->p_full[s][g & 1]);
+      }
+      steps += 2 * tiles;
+      done += items;
+      bar_sync(2 + s, 2 * kTileRows);  // (the last maxima have been read)
+      *mine = l;
+      bar_sync(2 + s, 2 * kTileRows);
+      l += *other;  // (each of the two adds the other's: the same sum)
+      tile_wait(&ct->pv_done[s][(done - 1) & 1], (done - 1) >> 1, dead);  // (the item two before is known to be done: S)
+      tc_fence_after();
+
+      // A unit that is cut leaves its pieces (O, maximum, sum) to the joining kernel.  One that is not is written here; with
+      // one row tile, stream 1 first hands its sums to stream 0 through the q buffers (every product that reads them is done
+      // once both streams' last are).
+      const bool cut_unit = u.tb - u.ta != u.tiles, joins = !cut_unit && !u.two;
+      float4* hand = reinterpret_cast<float4*>(q_buf) + half * (kD / 8) * kTileRows;
+      float f0 = 1.f, f1 = 0.f;
+      if (joins) {
+        if (s == 1) {
+          tile_wait(&ct->pv_done[0][(done - 1) & 1], (done - 1) >> 1, dead);
+          tc_fence_after();
+          if (half == 0) ct->hand[row] = make_float2(m, l);
+#pragma unroll
+          for (int c = 0; c < kD / 64; ++c) {
+            uint32_t x[32];
+            tmem_ld32(x, to + c * 32);
+            tmem_wait_ld(x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hand[(c * 8 + i) * kTileRows + row] = make_float4(
+                __uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3]));
+          }
+        }
+        bar_sync(1, kTileSoftmax);
+        if (s == 0) {
+          const float2 o = ct->hand[row];
+          const float mn = fmaxf(m, o.x);
+          f0 = m == -INFINITY ? 0.f : ex2(m - mn), f1 = o.x == -INFINITY ? 0.f : ex2(o.x - mn);
+          l = l * f0 + o.y * f1;
+          m = mn;
+        }
+      }
+      if (!(joins && s == 1)) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t slot = kv_tile_slot(blockIdx.x, u.ta == 0, s);
+#pragma unroll
+        for (int c = 0; c < kD / 64; ++c) {
+          uint32_t x[32];
+          tmem_ld32(x, to + c * 32);
+          tmem_wait_ld(x);
+          if (cut_unit) {
+            if (on) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                __stcg(a.part + (slot * (kD / 4) + half * (kD / 8) + c * 8 + i) * kTileRows + row,
+                       make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])));
+            }
+          } else if (exists) {
+            uint2* o = reinterpret_cast<uint2*>(a.o + out_row * kD + half * (kD / 2) + c * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (joins) v = hand[(c * 8 + i) * kTileRows + row];
+              const float y0 = fmaf(__uint_as_float(x[4 * i]), f0, v.x * f1), y1 = fmaf(__uint_as_float(x[4 * i + 1]), f0, v.y * f1);
+              const float y2 = fmaf(__uint_as_float(x[4 * i + 2]), f0, v.z * f1), y3 = fmaf(__uint_as_float(x[4 * i + 3]), f0, v.w * f1);
+              o[i] = on ? make_uint2(pack_bf16x2(y0 * inv, y1 * inv), pack_bf16x2(y2 * inv, y3 * inv)) : make_uint2(0u, 0u);
+            }
+          }
+        }
+        if (half == 0) {
+          if (cut_unit) __stcg(a.ml + slot * kTileRows + row, make_float2(m, l));
+          else if (exists && a.lse) a.lse[out_row] = on && l != 0.f ? (m - kTileTop + lg2(l)) * 0.69314718055994531f : -INFINITY;
+        }
+      }
+      tc_fence_before();
+      bar_sync(1, kTileSoftmax);  // the q buffers are written again by the next unit
+    }
+  }
+  __syncthreads();
+  if (warp == kTileMmaWarp) {
+    tc_fence_after();
+    tmem_free(0, 512);
+  }
+}
+
+// Joins the pieces that the tile kernel left, in the order of the tokens.  A launch of its own, after the tile kernel: joining
+// inside it, by the CTA that finishes a unit last, took 9 us of its end (fence, counter, then one thread per row reading
+// piece after piece); here every row has eight threads, and the search for the pieces runs before the wait for the tile kernel.
+// blockIdx = (32 rows of a row tile, kv head, sequence); a thread takes a row and kD / 8 of its values.
+constexpr int kJoinThreads = 256;
+template <int kD>
+__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const KvAttnArgs a, int grid) {
+  extern __shared__ int join_prefix[];
+  __shared__ int scan[kJoinThreads / 32];
+  // (The lengths are older than the tile kernel, which begins only when its own predecessor is done.)
+  const int64_t total = static_cast<int64_t>(kv_tile_prefix<kJoinThreads>(a, join_prefix, scan)) * a.c.kv_heads;
+  const int64_t ctas = kv_tile_ctas(total, grid);
+  const int b = blockIdx.z, h = blockIdx.y, rt = blockIdx.x * 32 / kTileUnitRows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const KvSpan sp = kv_span(a, b);
+  int t0 = 0, t1 = 0, before = 0;
+  for (int i = 0; i < rt; ++i) {
+    kv_tile_range(a, sp, i, t0, t1);
+    before += max(1, t1 - t0);
+  }
+  kv_tile_range(a, sp, rt, t0, t1);
+  const int tiles = max(1, t1 - t0);
+  const int64_t begin = static_cast<int64_t>(join_prefix[b]) * a.c.kv_heads + static_cast<int64_t>(join_prefix[b + 1] - join_prefix[b]) * h + before;
+  const int64_t c0 = ((begin + 1) * ctas - 1) / total, c1 = ((begin + tiles) * ctas - 1) / total;
+  const bool two = a.R * a.group - rt * kTileUnitRows > kTileRows;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (t1 <= t0 || c0 == c1) return;  // written by the tile kernel
+  const int rr = blockIdx.x * 32 + lane, r = rr / a.group;
+  if (r >= a.R) return;
+  const int row = rr % kTileRows, s0 = two ? rr % kTileUnitRows / kTileRows : 0, streams = two ? 1 : 2;
+  const int pieces = static_cast<int>(c1 - c0 + 1) * streams;
+  auto slot_of = [&](int p) { return kv_tile_slot(c0 + p / streams, p < streams, two ? s0 : p % streams); };
+  const int64_t out_row = (static_cast<int64_t>(b) * a.R + r) * a.heads + h * a.group + rr % a.group;
+  constexpr int kVecs = kD / 32;  // float4 of this thread
+  float4 acc[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, l = 0.f;
+  if (r < sp.n) {
+#pragma unroll 4
+    for (int p = 0; p < pieces; ++p) {
+      const float2 ml = ld_cg(a.ml + slot_of(p) * kTileRows + row);
+      m = fmaxf(m, ml.x);
+    }
+#pragma unroll 2
+    for (int p = 0; p < pieces; ++p) {
+      const int64_t slot = slot_of(p);
+      const float2 ml = ld_cg(a.ml + slot * kTileRows + row);
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+      l = fmaf(ml.y, f, l);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const float4 v = ld_cg(a.part + (slot * (kD / 4) + warp * kVecs + i) * kTileRows + row);
+        acc[i].x = fmaf(v.x, f, acc[i].x), acc[i].y = fmaf(v.y, f, acc[i].y);
+        acc[i].z = fmaf(v.z, f, acc[i].z), acc[i].w = fmaf(v.w, f, acc[i].w);
+      }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint2* o = reinterpret_cast<uint2*>(a.o + out_row * kD) + warp * kVecs;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i)
+    o[i] = r < sp.n ? make_uint2(pack_bf16x2(acc[i].x * inv, acc[i].y * inv), pack_bf16x2(acc[i].z * inv, acc[i].w * inv)) : make_uint2(0u, 0u);
+  if (a.lse && warp == 0) a.lse[out_row] = l != 0.f ? (m - kTileTop + lg2(l)) * 0.69314718055994531f : -INFINITY;
+}
+
+}  // namespace gguf_b200

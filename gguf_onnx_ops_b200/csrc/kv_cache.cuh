@@ -11,10 +11,39 @@
 
 namespace gguf_b200 {
 
-// The cache, its table and the lengths change between calls of one chain: they are read through the L2, not through
-// the read-only path, whose lines may be older than a programmatic launch's predecessor.
-__device__ __forceinline__ uint4 ldcg128(const void* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
-__device__ __forceinline__ uint2 ldcg64(const void* p) { return __ldcg(reinterpret_cast<const uint2*>(p)); }
+// Loads of what an earlier kernel of the same chain may have written: through the L2 (a line of the read-only path may be
+// older than a programmatic launch's predecessor), and volatile, since the compiler moves an ordinary cached-load intrinsic
+// across the wait for that predecessor.
+__device__ __forceinline__ int32_t ld_cg(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cg(const float* p) {
+  float v;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cg(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cg(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 ld_cg64(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_cg128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 
 struct KvPages {
   const int32_t* table;  // [B, table_cols] page of each sequence's i-th stretch of `page` tokens
@@ -22,15 +51,17 @@ struct KvPages {
   int table_cols, kv_heads, log2_page, D;
 };
 
+// Whether a table entry names a page of the cache; recorded where it does not.
+__device__ __forceinline__ bool kv_page_ok(const KvPages& c, int entry) {
+  if (entry >= 0 && entry < c.pages) return true;
+  record_device_error(kSiteBadCachePage);
+  return false;
+}
 // Page of stretch i of sequence b, or -1 (recorded) where the table or the page is out of range.
 __device__ __forceinline__ int64_t kv_page(const KvPages& c, int b, int i) {
   int p = -1;
-  if (i < c.table_cols) p = __ldcg(c.table + static_cast<int64_t>(b) * c.table_cols + i);
-  if (p < 0 || p >= c.pages) {
-    record_device_error(kSiteBadCachePage);
-    return -1;
-  }
-  return p;
+  if (i < c.table_cols) p = ld_cg(c.table + static_cast<int64_t>(b) * c.table_cols + i);
+  return kv_page_ok(c, p) ? p : -1;
 }
 
 struct KvWriteArgs {
@@ -69,8 +100,8 @@ __global__ void __launch_bounds__(kKvWriteThreads) kv_write_kernel(const KvWrite
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.z, h = blockIdx.y, which = blockIdx.x & 1, tid = threadIdx.x;
-  const int len = __ldcg(a.lens + b);
-  const int n = min(a.news ? __ldcg(a.news + b) : a.R, min(a.R, len));
+  const int len = ld_cg(a.lens + b);
+  const int n = min(a.news ? ld_cg(a.news + b) : a.R, min(a.R, len));
   const int first = len - n;
   const int lg = a.c.log2_page, i = (first >> lg) + (blockIdx.x >> 1);
   const int begin = i << lg;
@@ -91,13 +122,13 @@ __global__ void __launch_bounds__(kKvWriteThreads) kv_write_kernel(const KvWrite
   for (int j = 0; j < kKvWriteRegs; ++j) {
     const int p = tid + j * kKvWriteThreads;
     keep[j] = make_uint4(0, 0, 0, 0);
-    if (p < pieces) keep[j] = ldcg128(x + (p / per) * rs + (p % per) * 8);
+    if (p < pieces) keep[j] = ld_cg128(x + (p / per) * rs + (p % per) * 8);
   }
 #pragma unroll
   for (int j = 0; j < kKvWriteRegs; ++j)
     m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(m, keep[j].x), keep[j].y), keep[j].z), keep[j].w);
   for (int p = tid + kKvWriteRegs * kKvWriteThreads; p < pieces; p += kKvWriteThreads) {
-    const uint4 v = ldcg128(x + (p / per) * rs + (p % per) * 8);
+    const uint4 v = ld_cg128(x + (p / per) * rs + (p % per) * 8);
     m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(m, v.x), v.y), v.z), v.w);
   }
   m = max(m & 0xFFFFu, m >> 16);
@@ -136,7 +167,7 @@ __global__ void __launch_bounds__(kKvWriteThreads) kv_write_kernel(const KvWrite
   for (int j = 0; j < kKvWriteRegs; ++j)
     if (tid + j * kKvWriteThreads < pieces) put(tid + j * kKvWriteThreads, keep[j]);
   for (int p = tid + kKvWriteRegs * kKvWriteThreads; p < pieces; p += kKvWriteThreads)
-    put(p, ldcg128(x + (p / per) * rs + (p % per) * 8));
+    put(p, ld_cg128(x + (p / per) * rs + (p % per) * 8));
 }
 
 struct KvReadArgs {
@@ -169,15 +200,15 @@ __global__ void __launch_bounds__(kKvReadThreads) kv_read_kernel(const KvReadArg
   const int d = static_cast<int>(p % per);
   const int64_t rh = p / per;
   const int h = static_cast<int>(rh % a.c.kv_heads), r = static_cast<int>(rh / a.c.kv_heads);
-  const int pos = __ldcg(a.lens + b) - a.rows + r;
+  const int pos = ld_cg(a.lens + b) - a.rows + r;
   uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
   if (pos >= 0) {
     const int64_t page = kv_page(a.c, b, pos >> a.c.log2_page);
     if (page >= 0) {
       const int64_t at = page * a.c.kv_heads + h;
-      const float s = __ldcg(a.scales[which] + at);
+      const float s = ld_cg(a.scales[which] + at);
       const int in = pos & ((1 << a.c.log2_page) - 1);
-      const uint4 w = ldcg128(a.codes[which] + ((at << a.c.log2_page) + in) * a.c.D + d * 16);
+      const uint4 w = ld_cg128(a.codes[which] + ((at << a.c.log2_page) + in) * a.c.D + d * 16);
       const uint2 v0 = kv_values4(w.x, s), v1 = kv_values4(w.y, s), v2 = kv_values4(w.z, s), v3 = kv_values4(w.w, s);
       lo = make_uint4(v0.x, v0.y, v1.x, v1.y);
       hi = make_uint4(v2.x, v2.y, v3.x, v3.y);

@@ -9,6 +9,7 @@
 #include "qk_norm_rope.cuh"
 #include "kv_cache.cuh"
 #include "kv_attention.cuh"
+#include "kv_attention_tile.cuh"
 #include "draft_verify.cuh"
 
 namespace gguf_b200 {
@@ -58,66 +59,88 @@ cudaError_t run_rope(const RopeArgs& a, bool interleaved, cudaStream_t s) {
                      : launch_kernel(qk_norm_rope_kernel<kGL, kHeads, false>, grid, block, 0, s, a);
 }
 
-// Rows of query tokens and heads that share one kv head are taken kNT * 8 at a time.
-int attention_rows(int64_t rows) { return rows <= 8 ? 1 : 2; }
-
-template <int kD, int kNT>
-int64_t attention_part_bytes(int sms, int64_t* ml_off) {
-  using P = KvAttnPlan<kD, kNT>;
-  const int64_t ctas = static_cast<int64_t>(sms) * P::kCtas;
-  *ml_off = 2 * ctas * P::kFrags * 32 * 16;
-  return *ml_off + 2 * ctas * P::kRows * 8;
+// How a call's rows (query tokens x heads of one kv head) are taken: 8 or 16 at a time by the streaming kernel, or 256 at a
+// time by the tile kernel.
+struct AttentionPlan {
+  bool tile;
+  int rows;            // of a unit
+  int64_t row_tiles;   // units per kv head
+  int64_t counters(int64_t B, int64_t kv_heads) const { return tile ? 0 : B * kv_heads * row_tiles; }
+};
+AttentionPlan attention_plan(int64_t B, int64_t rows, int64_t D) {
+  AttentionPlan p;
+  p.tile = rows > 16 && (D == 64 || D == 128) && B <= kTileMaxBatch;
+  p.rows = p.tile ? kTileUnitRows : rows <= 8 ? 8 : 16;
+  p.row_tiles = (rows + p.rows - 1) / p.rows;
+  return p;
 }
 
-template <int kD, int kNT>
-int run_attention(KvAttnArgs& a, void* workspace, int sms, cudaStream_t s) {
-  using P = KvAttnPlan<kD, kNT>;
-  static std::atomic<uint64_t> done{0};
-  constexpr int kSmemMax = P::smem(kKvMaxBatch);
-  static_assert(kSmemMax <= 227 * 1024, "shared memory");
+template <typename Kernel>
+int raise_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_cuda_error("KvCacheAttention", e);
   if (!(done.load() >> (dev & 63) & 1)) {
-    e = cudaFuncSetAttribute(kv_attention_kernel<kD, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return set_cuda_error("KvCacheAttention", e);
     done.fetch_or(1ull << (dev & 63));
   }
-  int64_t ml_off;
-  attention_part_bytes<kD, kNT>(sms, &ml_off);
-  a.part = static_cast<float4*>(workspace);
-  a.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + ml_off);
-  e = launch_kernel(kv_attention_kernel<kD, kNT>, dim3(static_cast<unsigned>(sms * P::kCtas)), dim3(kKvThreads),
-                    P::smem(a.B), s, a);
-  return e == cudaSuccess ? GGUF_OK : set_cuda_error("KvCacheAttention launch", e);
+  return GGUF_OK;
 }
 
-// Calls f<D, NT>() for the instantiation that D and the rows take.
+// The streaming kernel for heads of kD values and kNT * 8 rows a unit.
+template <int kD, int kNT>
+struct Stream {
+  using P = KvAttnPlan<kD, kNT>;
+  static int64_t part_bytes(int sms) { return 2ll * sms * P::kCtas * P::kFrags * 32 * 16; }
+  static int64_t ml_bytes(int sms) { return 2ll * sms * P::kCtas * P::kRows * 8; }
+  static int run(const KvAttnArgs& a, int sms, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    static_assert(P::smem(kKvMaxBatch) <= 227 * 1024, "shared memory");
+    if (int rc = raise_smem(kv_attention_kernel<kD, kNT>, P::smem(kKvMaxBatch), done)) return rc;
+    cudaError_t e = launch_kernel(kv_attention_kernel<kD, kNT>, dim3(static_cast<unsigned>(sms * P::kCtas)), dim3(kKvThreads),
+                                  P::smem(a.B), s, a);
+    return e == cudaSuccess ? GGUF_OK : set_cuda_error("KvCacheAttention launch", e);
+  }
+};
+// The tile kernel.
+template <int kD>
+struct Tile {
+  using P = KvTilePlan<kD>;
+  static int64_t part_bytes(int sms) { return 4ll * sms * kTileRows * kD * 4; }
+  static int64_t ml_bytes(int sms) { return 4ll * sms * kTileRows * 8; }
+  static int run(const KvAttnArgs& a, int sms, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    static std::atomic<int> regs{0};
+    if (!regs.load()) {  // the kernel's warp groups share out what it is launched with
+      cudaFuncAttributes f;
+      cudaError_t e = cudaFuncGetAttributes(&f, kv_attention_tile_kernel<kD>);
+      if (e != cudaSuccess) return set_cuda_error("KvCacheAttention", e);
+      if (f.numRegs < kTileLaunchRegs) return set_error(GGUF_ERR_CUDA, "KvCacheAttention: built with too few registers");
+      regs.store(f.numRegs);
+    }
+    if (int rc = raise_smem(kv_attention_tile_kernel<kD>, P::smem(kTileMaxBatch), done)) return rc;
+    cudaError_t e = launch_kernel(kv_attention_tile_kernel<kD>, dim3(static_cast<unsigned>(sms)), dim3(kTileThreads), P::smem(a.B), s, a);
+    if (e != cudaSuccess) return set_cuda_error("KvCacheAttention launch", e);
+    const dim3 rows(static_cast<unsigned>((static_cast<int64_t>(a.R) * a.group + 31) / 32), static_cast<unsigned>(a.c.kv_heads), static_cast<unsigned>(a.B));
+    e = launch_kernel(kv_attention_join_kernel<kD>, rows, dim3(kJoinThreads), (a.B + 1) * sizeof(int), s, a, sms);
+    return e == cudaSuccess ? GGUF_OK : set_cuda_error("KvCacheAttention launch", e);
+  }
+};
+
+// Calls f with the kernel of a plan.
 template <typename F>
-auto attention_dispatch(int64_t D, int nt, F&& f) {
+auto attention_dispatch(const AttentionPlan& p, int64_t D, F&& f) {
+  if (p.tile) return D == 64 ? f(Tile<64>{}) : f(Tile<128>{});
+  const bool one = p.rows == 8;
   switch (D) {
-    case 64: return nt == 1 ? f.template operator()<64, 1>() : f.template operator()<64, 2>();
-    case 96: return nt == 1 ? f.template operator()<96, 1>() : f.template operator()<96, 2>();
-    case 128: return nt == 1 ? f.template operator()<128, 1>() : f.template operator()<128, 2>();
-    case 192: return nt == 1 ? f.template operator()<192, 1>() : f.template operator()<192, 2>();
-    default: return nt == 1 ? f.template operator()<256, 1>() : f.template operator()<256, 2>();
+    case 64: return one ? f(Stream<64, 1>{}) : f(Stream<64, 2>{});
+    case 96: return one ? f(Stream<96, 1>{}) : f(Stream<96, 2>{});
+    case 128: return one ? f(Stream<128, 1>{}) : f(Stream<128, 2>{});
+    case 192: return one ? f(Stream<192, 1>{}) : f(Stream<192, 2>{});
+    default: return one ? f(Stream<256, 1>{}) : f(Stream<256, 2>{});
   }
 }
-
-struct PartBytes {
-  int sms;
-  int64_t* off;
-  template <int kD, int kNT>
-  int64_t operator()() const { return attention_part_bytes<kD, kNT>(sms, off); }
-};
-struct RunAttention {
-  KvAttnArgs* a;
-  void* workspace;
-  int sms;
-  cudaStream_t s;
-  template <int kD, int kNT>
-  int operator()() const { return run_attention<kD, kNT>(*a, workspace, sms, s); }
-};
 
 int attention_shape(const char* op, int64_t B, int64_t R, int64_t heads, int64_t kv_heads) {
   if (B < 0 || B > kKvMaxBatch) return invalid(op, "batch must be in [0, 4096]");
@@ -223,11 +246,9 @@ int gguf_kv_cache_attention_workspace(int64_t B, int64_t R, int64_t heads, int64
   if (!known_dim(head_dim)) return invalid(op, "head_dim must be 64, 96, 128, 192 or 256");
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  const int64_t rows = R * (heads / kv_heads);
-  const int nt = attention_rows(rows);
-  int64_t off;
-  *bytes = attention_dispatch(head_dim, nt, PartBytes{sms, &off});
-  *counters = B * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
+  const AttentionPlan p = attention_plan(B, R * (heads / kv_heads), head_dim);
+  *bytes = attention_dispatch(p, head_dim, [&](auto k) { return k.part_bytes(sms) + k.ml_bytes(sms); });
+  *counters = p.counters(B, kv_heads);
   return GGUF_OK;
 }
 
@@ -249,9 +270,8 @@ int gguf_kv_cache_attention(const GgufKvCache* cache, const void* q, const int32
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   const int64_t group = heads / cache->kv_heads, rows = R * group;
-  const int nt = attention_rows(rows);
-  const int64_t row_tiles = (rows + 8 * nt - 1) / (8 * nt);
-  if (B * cache->kv_heads * row_tiles >= (1ll << 31)) return invalid(op, "too many rows");
+  const AttentionPlan p = attention_plan(B, rows, cache->head_dim);
+  if (B * cache->kv_heads * p.row_tiles >= (1ll << 31)) return invalid(op, "too many rows");
   a.k = static_cast<const int8_t*>(cache->k), a.v = static_cast<const int8_t*>(cache->v);
   a.ks = cache->k_scale, a.vs = cache->v_scale;
   a.q = static_cast<const bf16*>(q), a.o = static_cast<bf16*>(out), a.lse = lse;
@@ -260,9 +280,13 @@ int gguf_kv_cache_attention(const GgufKvCache* cache, const void* q, const int32
   a.scale_log2 = scale * 1.44269504088896341f;
   a.B = static_cast<int>(B), a.R = static_cast<int>(R), a.heads = static_cast<int>(heads), a.group = static_cast<int>(group);
   a.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
-  a.row_tiles = static_cast<int>(row_tiles);
+  a.row_tiles = static_cast<int>(p.row_tiles);
   a.counters = counters;
-  return attention_dispatch(cache->head_dim, nt, RunAttention{&a, workspace, sms, static_cast<cudaStream_t>(stream)});
+  return attention_dispatch(p, cache->head_dim, [&](auto k) {
+    a.part = static_cast<float4*>(workspace);
+    a.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + k.part_bytes(sms));
+    return k.run(a, sms, static_cast<cudaStream_t>(stream));
+  });
 }
 
 int gguf_draft_verify(const float* target, const float* draft_probs, const int32_t* draft, const float* u_accept,

@@ -10,7 +10,7 @@
 // for the kHeads heads that a group works on.
 #pragma once
 
-#include "common.cuh"
+#include "kv_cache.cuh"
 
 namespace gguf_b200 {
 
@@ -48,13 +48,13 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
   for (int i = 0; i < kHeads; ++i) {
     va[i] = vb[i] = make_uint2(0, 0);
     if (live && h0 + i < hn) {
-      va[i] = __ldcg(reinterpret_cast<const uint2*>(xr + i * a.D + oa));
-      vb[i] = __ldcg(reinterpret_cast<const uint2*>(xr + i * a.D + ob));
+      va[i] = ld_cg64(xr + i * a.D + oa);
+      vb[i] = ld_cg64(xr + i * a.D + ob);
     }
   }
   float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live && turns) {
-    int p = __ldcg(a.pos + t);
+    int p = ld_cg(a.pos + t);
     if (p < 0 || p >= a.max_pos) {
       record_device_error(kSiteBadPosition);
       p = 0;

@@ -135,6 +135,7 @@ def test_hidden_places_do_not_matter(cuda):
             t[table[0, :2].long()] = float("inf")
 
     run_case(cuda, 1, 1, 8, 2, 32, 128, [161], window=97, seed=12, edit=front)
+    run_case(cuda, 1, 20, 8, 2, 32, 128, [161 + 19], window=97, seed=12, edit=front)
 
 
 def test_marked_pages_are_seen(cuda):
