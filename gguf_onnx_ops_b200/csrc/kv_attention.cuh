@@ -13,8 +13,8 @@
 // besides the final bf16: 2^-12 of w_j, averaged over the tokens; 2^-40 of the largest weight for weights below 2^-29
 // of it, which is what the factor 2^15 is for.
 //
-// Work.  The cache positions of all (sequence, kv head, row tile) units are laid out in one line of 16-token tiles and cut
-// into equal slices, one per CTA, whatever the lengths are; lengths are read on the device, so a captured graph serves
+// Work.  The cache positions of all (sequence, kv head, row tile) units are laid out in one line of 16-token tiles, with a
+// stretch for each unit's own cost before them, and cut into equal slices, one per CTA, whatever the lengths are; lengths are read on the device, so a captured graph serves
 // any of them.  The eight warps of a CTA take its tiles in turn, each with its own statistics, and meet at the end of
 // the unit; a unit cut between CTAs leaves its pieces in the workspace, and the CTA that finishes last (a counter per
 // unit) joins them in order, so results do not depend on timing.
@@ -50,6 +50,9 @@ struct KvAttnArgs {
 constexpr int kKvWarps = 8;
 constexpr int kKvThreads = kKvWarps * 32;
 constexpr int kKvTile = 16;
+// What a unit costs besides its tiles (rows read, warps joined, a result written), in tiles: the slices count it, or the CTAs
+// that meet many short sequences end last (64 sequences of 131 to 8009 tokens: 129 us without, 119 with 6, 101 with 24).
+constexpr int kKvUnitCost = 32;
 constexpr int kKvMaxBatch = 4096;
 constexpr float kKvTop = 15.f;  // the largest weight is 2^15, the top of f16's range
 
@@ -142,7 +145,7 @@ struct KvAttnPlan {
   static constexpr int kOBytes = kKvWarps * kFrags * 32 * 16;
   static constexpr int kRowBytes = kRows * (4 + 4 + 4) + kKvWarps * kRows * 8;
   static constexpr int smem(int B) { return kQBytes + kOBytes + kRowBytes + 64 + (B + 1) * 4; }
-  static constexpr int kCtas = kNT == 1 && kD <= 128 ? 2 : 1;
+  static constexpr int kCtas = kD == 64 ? (kNT == 1 ? 3 : 2) : kD <= 128 ? 2 : 1;  // registers leave room for these
 };
 
 template <int kD, int kNT>
@@ -169,7 +172,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
     int n = 0;
     if (b0 + tid < a.B) {
       const KvSpan s = kv_span(a, b0 + tid);
-      n = max(1, s.t1 - s.t0);
+      n = kKvUnitCost + max(1, s.t1 - s.t0);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
   }
   const int per_seq = a.c.kv_heads * a.row_tiles;
   const int64_t total = static_cast<int64_t>(carry) * per_seq;
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + kKvWarps - 1) / kKvWarps);
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + 15) / 16);  // (no less than a tile a warp, on the whole)
   if (blockIdx.x >= ctas) return;
   int64_t at = total * blockIdx.x / ctas;
   const int64_t end = total * (blockIdx.x + 1) / ctas;
@@ -202,13 +205,48 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
       if (static_cast<int64_t>(prefix[mid]) * per_seq <= at) b = mid; else hi = mid;
     }
     const KvSpan sp = kv_span(a, b);
-    const int tiles = max(1, sp.t1 - sp.t0);
+    const int tiles = max(1, sp.t1 - sp.t0), span = kKvUnitCost + tiles;
     const int64_t in_seq = at - static_cast<int64_t>(prefix[b]) * per_seq;
-    const int hr = static_cast<int>(in_seq / tiles), ta = static_cast<int>(in_seq % tiles);
+    const int hr = static_cast<int>(in_seq / span), in_unit = static_cast<int>(in_seq % span);
     const int h = hr / a.row_tiles, rt = hr % a.row_tiles;
-    const int tb = static_cast<int>(min(static_cast<int64_t>(tiles), ta + (end - at)));
-    const int64_t unit_begin = at - ta;
-    at += tb - ta;
+    const int64_t first_tile = at - in_unit + kKvUnitCost;  // where the unit's tiles begin in the line
+    const int taken = static_cast<int>(min(static_cast<int64_t>(span - in_unit), end - at));
+    const int ta = max(0, in_unit - kKvUnitCost), tb = in_unit + taken - kKvUnitCost;
+    at += taken;
+    if (tb <= ta) continue;  // the slice ends within the unit's cost
+
+    // The warp's first tile on its way.
+    uint32_t kw[2][P::kSteps] = {}, vw[4][kD / 32] = {};
+    uint32_t ks = 0, vs = 0;  // bits of the tile's scales
+    const int stop = min(sp.t0 + tb, sp.t1);
+    int tile = sp.t0 + ta + warp;
+    const int lg = a.c.log2_page, in_page = (1 << lg) - 1;
+    const int32_t* table = a.c.table + static_cast<int64_t>(b) * a.c.table_cols;  // (positions below len lie in it)
+    uint32_t entry = 0, entry_next = 0;  // pages of `tile` and of this warp's next tile
+    auto page_of = [&](uint32_t e) { return static_cast<int64_t>(kv_page_ok(a.c, static_cast<int>(e)) ? e : 0); };
+    auto row0 = [&](int64_t page, int tl) {
+      return ((((page * a.c.kv_heads + h) << lg) + ((tl * kKvTile) & in_page))) * kD;
+    };
+    auto load_k = [&](int64_t page, int tl, bool on) {
+      const int8_t* p = a.k + row0(page, tl) + t * P::kKPiece;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < kD / (4 * P::kKPiece); ++j)
+          load_codes_if<P::kKPiece>(&kw[r][j * (P::kKPiece / 4)], p + (g + 8 * r) * kD + j * 4 * P::kKPiece, on);
+      ld_if(ks, a.ks + page * a.c.kv_heads + h, on);
+      ld_if(vs, a.vs + page * a.c.kv_heads + h, on);
+    };
+    auto load_v = [&](int64_t page, int tl, bool on) {
+      const int8_t* p = a.v + row0(page, tl) + g * (kD / 8);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_codes_if<kD / 8>(vw[r], p + (2 * t + (r & 1) + 8 * (r >> 1)) * kD, on);
+    };
+    ld_if(entry, table + ((tile * kKvTile) >> lg), tile < stop);
+    ld_if(entry_next, table + (((tile + kKvWarps) * kKvTile) >> lg), tile + kKvWarps < stop);
+    int64_t page = page_of(entry);
+    load_k(page, tile, tile < stop);
+    load_v(page, tile, tile < stop);
 
     // Rows: q as f16 fragments, their limits.
     for (int n = warp; n < P::kRows; n += kKvWarps) {
@@ -264,38 +302,6 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
     }
     all_lo = __reduce_max_sync(0xffffffffu, all_lo);
     all_hi = __reduce_min_sync(0xffffffffu, all_hi);
-
-    uint32_t kw[2][P::kSteps] = {}, vw[4][kD / 32] = {};
-    uint32_t ks = 0, vs = 0;  // bits of the tile's scales
-    const int stop = min(sp.t0 + tb, sp.t1);
-    int tile = sp.t0 + ta + warp;
-    const int lg = a.c.log2_page, in_page = (1 << lg) - 1;
-    const int32_t* table = a.c.table + static_cast<int64_t>(b) * a.c.table_cols;  // (positions below len lie in it)
-    uint32_t entry = 0, entry_next = 0;  // pages of `tile` and of this warp's next tile
-    auto page_of = [&](uint32_t e) { return static_cast<int64_t>(kv_page_ok(a.c, static_cast<int>(e)) ? e : 0); };
-    auto row0 = [&](int64_t page, int tl) {
-      return ((((page * a.c.kv_heads + h) << lg) + ((tl * kKvTile) & in_page))) * kD;
-    };
-    auto load_k = [&](int64_t page, int tl, bool on) {
-      const int8_t* p = a.k + row0(page, tl) + t * P::kKPiece;
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int j = 0; j < kD / (4 * P::kKPiece); ++j)
-          load_codes_if<P::kKPiece>(&kw[r][j * (P::kKPiece / 4)], p + (g + 8 * r) * kD + j * 4 * P::kKPiece, on);
-      ld_if(ks, a.ks + page * a.c.kv_heads + h, on);
-      ld_if(vs, a.vs + page * a.c.kv_heads + h, on);
-    };
-    auto load_v = [&](int64_t page, int tl, bool on) {
-      const int8_t* p = a.v + row0(page, tl) + g * (kD / 8);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) load_codes_if<kD / 8>(vw[r], p + (2 * t + (r & 1) + 8 * (r >> 1)) * kD, on);
-    };
-    ld_if(entry, table + ((tile * kKvTile) >> lg), tile < stop);
-    ld_if(entry_next, table + (((tile + kKvWarps) * kKvTile) >> lg), tile + kKvWarps < stop);
-    int64_t page = page_of(entry);
-    load_k(page, tile, tile < stop);
-    load_v(page, tile, tile < stop);
 
     while (tile < stop) {
       const int next = tile + kKvWarps;
@@ -397,8 +403,8 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
     __syncthreads();
 
     // Piece or whole?  A piece goes to slot 0 of this CTA when its unit began in an earlier one, else to slot 1.
-    const int64_t c_first = ((unit_begin + 1) * ctas - 1) / total;
-    const int64_t c_last = ((unit_begin + tiles) * ctas - 1) / total;
+    const int64_t c_first = ((first_tile + 1) * ctas - 1) / total;
+    const int64_t c_last = ((first_tile + tiles) * ctas - 1) / total;
     const int pieces = static_cast<int>(c_last - c_first) + 1;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (ta > 0 ? 0 : 1);
     const int64_t unit = (static_cast<int64_t>(b) * a.c.kv_heads + h) * a.row_tiles + rt;

@@ -37,6 +37,7 @@ constexpr int kTileTokens = 128;          // what the work is cut by
 constexpr int kTileStep = 64;             // tokens of a step
 constexpr int kTileMaxBatch = 2048;       // what the shared memory leaves room for (a larger batch is streamed)
 constexpr int kTileBufs = 3;              // K and V buffers
+constexpr int kTileUnitCost = 4;          // of a unit besides its tiles, in tiles (kKvUnitCost)
 constexpr int kTileRows = 128;            // of one stream
 constexpr int kTileUnitRows = 2 * kTileRows;
 constexpr float kTileTop = 11.f, kTileGrow = 4.f;  // weights start at 2^11 and may grow to 2^15
@@ -85,9 +86,9 @@ __device__ __forceinline__ void kv_tile_range(const KvAttnArgs& a, const KvSpan&
 
 struct KvTileUnit {
   KvSpan sp;
-  int b, h, rt, t0, ta, tb, tiles;  // token tiles t0 + ta .. t0 + tb - 1 of this CTA (tb == ta + 1 with nothing to do: work false)
-  int64_t begin;
-  bool work, two;  // two: two row tiles
+  int b, h, rt, t0, ta, tb, tiles;  // token tiles t0 + ta .. t0 + tb - 1 of this CTA, of `tiles`
+  int taken;                        // how far the slice has come with it
+  bool mine, work, two;             // mine: tiles are this CTA's; work: rows see something; two: two row tiles
 };
 __device__ __forceinline__ KvTileUnit kv_tile_unit(const KvAttnArgs& a, const int* prefix, int64_t at, int64_t end) {
   KvTileUnit u;
@@ -105,13 +106,14 @@ __device__ __forceinline__ KvTileUnit kv_tile_unit(const KvAttnArgs& a, const in
   for (u.rt = 0;; ++u.rt) {
     kv_tile_range(a, u.sp, u.rt, u.t0, t1);
     u.tiles = max(1, t1 - u.t0);
-    if (rem < u.tiles || u.rt + 1 >= a.row_tiles) break;
-    rem -= u.tiles;
+    if (rem < kTileUnitCost + u.tiles || u.rt + 1 >= a.row_tiles) break;
+    rem -= kTileUnitCost + u.tiles;
   }
-  u.ta = rem;
-  u.tb = static_cast<int>(min(static_cast<int64_t>(u.tiles), rem + (end - at)));
-  u.begin = at - rem;
-  u.work = t1 > u.t0;
+  u.taken = static_cast<int>(min(static_cast<int64_t>(kTileUnitCost + u.tiles - rem), end - at));
+  u.ta = max(0, rem - kTileUnitCost);
+  u.tb = rem + u.taken - kTileUnitCost;
+  u.mine = u.tb > u.ta;
+  u.work = u.mine && t1 > u.t0;
   u.two = a.R * a.group - u.rt * kTileUnitRows > kTileRows;
   return u;
 }
@@ -128,7 +130,7 @@ __device__ __forceinline__ int kv_tile_prefix(const KvAttnArgs& a, int* prefix, 
       for (int rt = 0; rt < a.row_tiles; ++rt) {
         int t0, t1;
         kv_tile_range(a, s, rt, t0, t1);
-        n += max(1, t1 - t0);
+        n += kTileUnitCost + max(1, t1 - t0);
       }
     }
 #pragma unroll
@@ -150,7 +152,7 @@ __device__ __forceinline__ int kv_tile_prefix(const KvAttnArgs& a, int* prefix, 
   return carry;
 }
 __device__ __forceinline__ int64_t kv_tile_ctas(int64_t total, int grid) {
-  return min(static_cast<int64_t>(grid), (total + 1) / 2);
+  return min(static_cast<int64_t>(grid), (total + kTileUnitCost + 1) / (kTileUnitCost + 2));
 }
 // Workspace slot of CTA c's piece of stream s: every CTA cuts at most one unit at its front and one at its end.
 __device__ __forceinline__ int64_t kv_tile_slot(int64_t c, bool begins, int s) { return (2 * c + (begins ? 1 : 0)) * 2 + s; }
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     uint32_t slot = is_v ? 1 : 0, slot_use = 0, buf = 0, use = 0;
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
-      at += u.tb - u.ta;
+      at += u.taken;
       if (!u.work) continue;
       for (int left = 2 * (u.tb - u.ta); left > 0; --left) {
         tile_wait(&ct->raw_full[slot], slot_use, dead);
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     uint32_t n = 0;  // staged steps
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
-      at += u.tb - u.ta;
+      at += u.taken;
       if (!u.work) continue;
       const int st_end = 2 * (u.t0 + u.tb);
       const int32_t* table = a.c.table + static_cast<int64_t>(u.b) * a.c.table_cols;  // (positions below len lie in it)
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     uint32_t steps = 0;
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
-      at += u.tb - u.ta;
+      at += u.taken;
       if (!u.work) continue;
       const int st_end = 2 * (u.t0 + u.tb);
       const int32_t* table = a.c.table + static_cast<int64_t>(u.b) * a.c.table_cols;
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     uint32_t steps = 0, done = 0, units = 0;  // of the units before: steps, items of a stream, units
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
-      at += u.tb - u.ta;
+      at += u.taken;
       if (!u.work) continue;
       const int tiles = u.tb - u.ta, items = u.two ? 2 * tiles : tiles;
       tile_wait(&ct->q_full[0], units, dead);
@@ -413,12 +415,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     uint32_t steps = 0, done = 0;
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
-      at += u.tb - u.ta;
+      at += u.taken;
       const int rr = u.rt * kTileUnitRows + (u.two ? s : 0) * kTileRows + row, r = rr / a.group;
       const bool on = r < u.sp.n, exists = r < a.R;
       const int64_t out_row = (static_cast<int64_t>(u.b) * a.R + r) * a.heads + u.h * a.group + rr % a.group;
-      if (!u.work) {  // none of the unit's rows sees anything
-        if (exists && (u.two || s == 0)) {
+      if (!u.work) {  // none of the unit's rows sees anything (or the slice ends before its tiles)
+        if (u.mine && exists && (u.two || s == 0)) {
           uint4* o = reinterpret_cast<uint4*>(a.o + out_row * kD) + half * (kD / 16);
           for (int i = 0; i < kD / 16; ++i) o[i] = make_uint4(0, 0, 0, 0);
           if (a.lse && half == 0) a.lse[out_row] = -INFINITY;
@@ -643,12 +645,13 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
   int t0 = 0, t1 = 0, before = 0;
   for (int i = 0; i < rt; ++i) {
     kv_tile_range(a, sp, i, t0, t1);
-    before += max(1, t1 - t0);
+    before += kTileUnitCost + max(1, t1 - t0);
   }
   kv_tile_range(a, sp, rt, t0, t1);
   const int tiles = max(1, t1 - t0);
   const int64_t begin = static_cast<int64_t>(join_prefix[b]) * a.c.kv_heads + static_cast<int64_t>(join_prefix[b + 1] - join_prefix[b]) * h + before;
-  const int64_t c0 = ((begin + 1) * ctas - 1) / total, c1 = ((begin + tiles) * ctas - 1) / total;
+  const int64_t first = begin + kTileUnitCost;  // of the unit's tiles
+  const int64_t c0 = ((first + 1) * ctas - 1) / total, c1 = ((first + tiles) * ctas - 1) / total;
   const bool two = a.R * a.group - rt * kTileUnitRows > kTileRows;
   pdl_wait();
   pdl_launch_dependents();
