@@ -7,7 +7,7 @@
 // numbers do not depend on their order, so however the row is cut the token is the same.  Where T is 0 the draw is
 // made from p_n instead, and where that is empty too the token is -1.
 //
-// One cluster of eight CTAs per sequence: each sums its eighth of the row (two fp32 reads a token, nothing kept), the
+// One cluster of up to eight CTAs per sequence: each sums its part of the row (two fp32 reads a token, nothing kept), the
 // CTAs' totals meet through distributed shared memory, and the one warp whose stretch holds the target reads that stretch
 // again (from the L2) to find the token.
 #pragma once
@@ -28,26 +28,28 @@ struct DraftArgs {
   int R, V;
 };
 
-constexpr int kDraftCtas = 8;
+constexpr int kDraftCtas = 8;   // of a sequence, at most
 constexpr int kDraftThreads = 512;
 constexpr int kDraftWarps = kDraftThreads / 32;
 constexpr int kDraftMax = 32;
 
-__device__ __forceinline__ unsigned long long draft_mass(float p, float q) {
-  const float w = fminf(fmaxf(__fsub_rn(p, q), 0.f), 1.f);  // NaN: 0
-  return __float2ull_rz(w * 274877906944.0f);
+constexpr int kDraftBatch = 4;  // steps whose loads are on their way at once
+
+__device__ __forceinline__ float draft_weight(uint32_t p, uint32_t q) {
+  return fminf(fmaxf(__fsub_rn(__uint_as_float(p), __uint_as_float(q)), 0.f), 1.f);  // NaN: 0
 }
+__device__ __forceinline__ unsigned long long draft_mass(float w) { return __float2ull_rz(w * 274877906944.0f); }
 
 // kVec values per lane and load (4 needs V % 4 == 0 and 16-byte aligned rows).
 template <int kVec>
-__global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThreads) draft_verify_kernel(const DraftArgs a) {
+__global__ void __launch_bounds__(kDraftThreads, 2) draft_verify_kernel(const DraftArgs a) {
   namespace cg = cooperative_groups;
   __shared__ unsigned long long warp_sum[kDraftWarps], cta_sum[2];
   pdl_wait();
   pdl_launch_dependents();
   auto cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int b = blockIdx.x / kDraftCtas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+  const int b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n_drafts = a.drafts ? max(0, min(a.R, ld_cg(a.drafts + b))) : a.R;
   const int64_t V = a.V;
 
@@ -75,30 +77,30 @@ __global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThrea
   const float* q = rejected && a.q ? a.q + (static_cast<int64_t>(b) * a.R + n) * V : nullptr;
   const int skip = rejected && !a.q ? x_n : -1;  // the token a certain draft takes out of the row
   // The row in warp stretches of whole 32 kVec-value steps.
-  const int step = 32 * kVec, steps = (a.V + step - 1) / step, all_warps = kDraftCtas * kDraftWarps;
+  const int step = 32 * kVec, steps = (a.V + step - 1) / step, all_warps = ctas * kDraftWarps;
   const int w_id = rank * kDraftWarps + warp;
   const int s0 = static_cast<int>(static_cast<int64_t>(steps) * w_id / all_warps);
   const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (w_id + 1) / all_warps);
-  auto masses = [&](int s, bool with_q, unsigned long long (&w)[kVec]) {
-    const int v = s * step + lane * kVec;
-    float pv[kVec], qv[kVec];
+  // w of this lane's values of kDraftBatch steps from s on (0 past the warp's stretch).
+  auto weights = [&](int s, bool with_q, float (&w)[kDraftBatch][kVec]) {
+    alignas(16) uint32_t pw[kDraftBatch][kVec] = {}, qw[kDraftBatch][kVec] = {};
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) pv[i] = qv[i] = 0.f;
-    if (v < a.V) {
+    for (int k = 0; k < kDraftBatch; ++k) {
+      const int v = (s + k) * step + lane * kVec;
+      const bool in = s + k < s1 && v < a.V;
       if constexpr (kVec == 4) {
-        const float4 f = ld_cg(reinterpret_cast<const float4*>(p + v));
-        pv[0] = f.x, pv[1] = f.y, pv[2] = f.z, pv[3] = f.w;
-        if (q && with_q) {
-          const float4 e = ld_cg(reinterpret_cast<const float4*>(q + v));
-          qv[0] = e.x, qv[1] = e.y, qv[2] = e.z, qv[3] = e.w;
-        }
+        ld_cg128_if(*reinterpret_cast<uint4*>(pw[k]), p + v, in);
+        ld_cg128_if(*reinterpret_cast<uint4*>(qw[k]), q + v, in && q && with_q);
       } else {
-        pv[0] = ld_cg(p + v);
-        if (q && with_q) qv[0] = ld_cg(q + v);
+        ld_cg32_if(pw[k][0], p + v, in);
+        ld_cg32_if(qw[k][0], q + v, in && q && with_q);
       }
     }
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) w[i] = with_q && v + i == skip ? 0ull : draft_mass(pv[i], qv[i]);
+    for (int k = 0; k < kDraftBatch; ++k)
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        w[k][i] = with_q && (s + k) * step + lane * kVec + i == skip ? 0.f : draft_weight(pw[k][i], qw[k][i]);
   };
 
   int token = -1;
@@ -107,12 +109,13 @@ __global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThrea
   for (int pass = 0; pass < 2; ++pass) {  // pass 1: the residual is empty, draw from p_n
     const bool with_q = pass == 0;
     unsigned long long sum = 0;
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-      unsigned long long w[kVec];
-      masses(s, with_q, w);
+    for (int s = s0; s < s1; s += kDraftBatch) {
+      float w[kDraftBatch][kVec];
+      weights(s, with_q, w);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) sum += w[i];
+      for (int k = 0; k < kDraftBatch; ++k)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sum += draft_mass(w[k][i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -125,8 +128,7 @@ __global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThrea
     }
     cluster.sync();
     unsigned long long total = 0, before = 0;
-#pragma unroll
-    for (int r = 0; r < kDraftCtas; ++r) {
+    for (int r = 0; r < ctas; ++r) {
       const unsigned long long c = *cluster.map_shared_rank(&cta_sum[pass], r);
       total += c;
       if (r < rank) before += c;
@@ -143,31 +145,36 @@ __global__ void __cluster_dims__(kDraftCtas, 1, 1) __launch_bounds__(kDraftThrea
     mine = false;
     if (before <= target && target < before + sum) {  // in this warp's stretch
       unsigned long long run = before;
-      for (int s = s0; s < s1; ++s) {
-        unsigned long long w[kVec], c = 0;
-        masses(s, with_q, w);
+      bool found = false;
+      for (int s = s0; s < s1 && !found; s += kDraftBatch) {
+        float w[kDraftBatch][kVec];
+        weights(s, with_q, w);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) c += w[i];
-        unsigned long long incl = c;
+        for (int k = 0; k < kDraftBatch; ++k) {
+          if (found) continue;
+          unsigned long long c = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, run + incl > target);
-        if (hit) {
-          mine = lane == __ffs(hit) - 1;
-          unsigned long long low = run + incl - c;
-          for (int i = 0; i < kVec; ++i) {
-            low += w[i];
-            if (low > target) {
-              token = s * step + lane * kVec + i;
-              break;
+          for (int i = 0; i < kVec; ++i) c += draft_mass(w[k][i]);
+          unsigned long long incl = c;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+          }
+          const unsigned hit = __ballot_sync(0xffffffffu, run + incl > target);
+          if (hit) {
+            found = true;
+            mine = lane == __ffs(hit) - 1;
+            unsigned long long low = run + incl - c;
+            bool past = false;
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+              low += draft_mass(w[k][i]);
+              if (!past && low > target) token = (s + k) * step + lane * kVec + i, past = true;
             }
           }
-          break;
+          run += __shfl_sync(0xffffffffu, incl, 31);
         }
-        run += __shfl_sync(0xffffffffu, incl, 31);
       }
     }
     break;

@@ -89,12 +89,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Predicated loads that leave their registers alone where `on` is false.  Prefetches for the next turn of a loop are written
-// with them: behind a branch the compiler merges the two values with moves, which wait for the load.
-__device__ __forceinline__ void ld_if(uint32_t& w, const void* p, bool on) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p ld.global.cg.u32 %0, [%1];\n}\n" : "+r"(w) : "l"(p), "r"(on ? 1u : 0u) : "memory");
-}
-// kBytes consecutive bytes (4, 8 or 16 at a time) of a cache page into words; read once, kept out of L1.
+// kBytes consecutive bytes (4, 8 or 16 at a time) of a cache page into words (predicated as ld_cg32_if); read
+// once, kept out of L1.
 template <int kBytes>
 __device__ __forceinline__ void load_codes_if(uint32_t* w, const int8_t* p, bool on) {
   const uint32_t c = on ? 1u : 0u;
@@ -234,16 +230,16 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
 #pragma unroll
         for (int j = 0; j < kD / (4 * P::kKPiece); ++j)
           load_codes_if<P::kKPiece>(&kw[r][j * (P::kKPiece / 4)], p + (g + 8 * r) * kD + j * 4 * P::kKPiece, on);
-      ld_if(ks, a.ks + page * a.c.kv_heads + h, on);
-      ld_if(vs, a.vs + page * a.c.kv_heads + h, on);
+      ld_cg32_if(ks, a.ks + page * a.c.kv_heads + h, on);
+      ld_cg32_if(vs, a.vs + page * a.c.kv_heads + h, on);
     };
     auto load_v = [&](int64_t page, int tl, bool on) {
       const int8_t* p = a.v + row0(page, tl) + g * (kD / 8);
 #pragma unroll
       for (int r = 0; r < 4; ++r) load_codes_if<kD / 8>(vw[r], p + (2 * t + (r & 1) + 8 * (r >> 1)) * kD, on);
     };
-    ld_if(entry, table + ((tile * kKvTile) >> lg), tile < stop);
-    ld_if(entry_next, table + (((tile + kKvWarps) * kKvTile) >> lg), tile + kKvWarps < stop);
+    ld_cg32_if(entry, table + ((tile * kKvTile) >> lg), tile < stop);
+    ld_cg32_if(entry_next, table + (((tile + kKvWarps) * kKvTile) >> lg), tile + kKvWarps < stop);
     int64_t page = page_of(entry);
     load_k(page, tile, tile < stop);
     load_v(page, tile, tile < stop);
@@ -323,7 +319,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
       page = page_of(entry_next);  // (read a tile ahead; page 0 where there is no next tile)
       load_k(page, next, more);
       entry_next = more ? entry_next : 0;
-      ld_if(entry_next, table + (((next + kKvWarps) * kKvTile) >> lg), next + kKvWarps < stop);
+      ld_cg32_if(entry_next, table + (((next + kKvWarps) * kKvTile) >> lg), next + kKvWarps < stop);
 
       const float lv = lg2(vs_now), inv_v = __fdividef(1.0f, vs_now);
       const int p0 = tile * kKvTile;

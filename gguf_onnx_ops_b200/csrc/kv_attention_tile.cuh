@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       auto wanted = [&](int st) { return lane < chunks && st < st_end && st * kTileStep + lane * chunk < u.sp.len; };
       auto entry_of = [&](int st) {
         uint32_t e = 0;
-        ld_if(e, table + ((st * kTileStep + lane * chunk) >> lg), wanted(st));
+        ld_cg32_if(e, table + ((st * kTileStep + lane * chunk) >> lg), wanted(st));
         return e;
       };
       auto copy = [&](const int8_t* codes, int st, uint32_t entry, bool copies) {
@@ -301,12 +301,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       auto entry_of = [&](int st) {
         const int pos = st * kTileStep + (lane & 3) * 16;
         uint32_t e = 0xFFFFFFFFu;
-        ld_if(e, table + (pos >> lg), st < st_end && pos < u.sp.len);
+        ld_cg32_if(e, table + (pos >> lg), st < st_end && pos < u.sp.len);
         return e;
       };
       auto scale_of = [&](uint32_t e) {
         uint32_t w = 0;
-        ld_if(w, (lane < 4 ? a.ks : a.vs) + static_cast<int64_t>(static_cast<int>(e)) * a.c.kv_heads + u.h, lane < 8 && e < a.c.pages);
+        ld_cg32_if(w, (lane < 4 ? a.ks : a.vs) + static_cast<int64_t>(static_cast<int>(e)) * a.c.kv_heads + u.h, lane < 8 && e < a.c.pages);
         return w;
       };
       int st = 2 * (u.t0 + u.ta);

@@ -45,6 +45,20 @@ __device__ __forceinline__ uint4 ld_cg128(const void* p) {
   return v;
 }
 
+// Predicated forms, which leave the registers alone where `on` is false: behind a branch the compiler merges the two
+// values with moves, which wait for the load.
+__device__ __forceinline__ void ld_cg32_if(uint32_t& w, const void* p, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p ld.global.cg.u32 %0, [%1];\n}\n" : "+r"(w) : "l"(p), "r"(on ? 1u : 0u) : "memory");
+}
+__device__ __forceinline__ void ld_cg64_if(uint2& v, const void* p, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %3, 0;\n @p ld.global.cg.v2.u32 {%0, %1}, [%2];\n}\n" : "+r"(v.x), "+r"(v.y)
+               : "l"(p), "r"(on ? 1u : 0u) : "memory");
+}
+__device__ __forceinline__ void ld_cg128_if(uint4& v, const void* p, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n @p ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];\n}\n"
+               : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "l"(p), "r"(on ? 1u : 0u) : "memory");
+}
+
 struct KvPages {
   const int32_t* table;  // [B, table_cols] page of each sequence's i-th stretch of `page` tokens
   int64_t pages;
@@ -94,48 +108,55 @@ __device__ __forceinline__ uint32_t kv_rescale4(uint32_t w, float ratio) {
 }
 __device__ __forceinline__ uint32_t abs_max_bf16x2(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7FFF7FFFu); }
 
-// One CTA per (touched page, head, K or V) of a sequence: blockIdx = (page of the call * 2 + which, head, sequence).
+// One CTA per (touched page, head, K or V) of a sequence: blockIdx = (page of the call * 2 + which, head, sequence).  The
+// call's tokens of the page stay in registers between the maximum and the codes (16 KB at 64 tokens of 128 values); loads
+// that do not depend on one another are issued before any is used.
+template <int kD>
 __global__ void __launch_bounds__(kKvWriteThreads) kv_write_kernel(const KvWriteArgs a) {
+  constexpr int kPer = kD / 8;  // 16-byte pieces of a token
   __shared__ uint32_t red[kKvWriteThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.z, h = blockIdx.y, which = blockIdx.x & 1, tid = threadIdx.x;
-  const int len = ld_cg(a.lens + b);
-  const int n = min(a.news ? ld_cg(a.news + b) : a.R, min(a.R, len));
+  int len = ld_cg(a.lens + b), n = a.R;
+  if (a.news) n = ld_cg(a.news + b);
+  n = min(n, min(a.R, len));
   const int first = len - n;
   const int lg = a.c.log2_page, i = (first >> lg) + (blockIdx.x >> 1);
   const int begin = i << lg;
   if (n <= 0 || begin >= len) return;
-  const int64_t page = kv_page(a.c, b, i);
-  if (page < 0) return;
+  int entry = -1;
+  if (i < a.c.table_cols) entry = ld_cg(a.c.table + static_cast<int64_t>(b) * a.c.table_cols + i);
   const int t0 = max(first, begin), t1 = min(len, begin + (1 << lg));
-  const int per = a.c.D >> 3, pieces = (t1 - t0) * per;
-  const bf16* x = a.x[which] + b * a.stride_b[which] + (t0 - first) * a.stride_r[which] + h * a.c.D;
-  const int64_t rs = a.stride_r[which];
-  const int64_t at = page * a.c.kv_heads + h;
-  int8_t* codes = a.codes[which] + ((at << lg) * a.c.D);
-  float* scale_p = a.scales[which] + at;
+  const int pieces = (t1 - t0) * kPer;
+  const int64_t rs = which ? a.stride_r[1] : a.stride_r[0];
+  const bf16* x = (which ? a.x[1] : a.x[0]) + b * (which ? a.stride_b[1] : a.stride_b[0]) + (t0 - first) * rs + h * kD;
 
   uint4 keep[kKvWriteRegs];
-  uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < kKvWriteRegs; ++j) {
     const int p = tid + j * kKvWriteThreads;
     keep[j] = make_uint4(0, 0, 0, 0);
-    if (p < pieces) keep[j] = ld_cg128(x + (p / per) * rs + (p % per) * 8);
+    ld_cg128_if(keep[j], x + (p / kPer) * rs + (p % kPer) * 8, p < pieces);
   }
+  if (!kv_page_ok(a.c, entry)) return;
+  const int64_t at = static_cast<int64_t>(entry) * a.c.kv_heads + h;
+  int8_t* codes = (which ? a.codes[1] : a.codes[0]) + ((at << lg) * kD);
+  float* scale_p = (which ? a.scales[1] : a.scales[0]) + at;
+  const bool older = t0 > begin;
+  float was = 0.f;
+  if (older) was = ld_cg(scale_p);
+  uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < kKvWriteRegs; ++j)
     m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(m, keep[j].x), keep[j].y), keep[j].z), keep[j].w);
   for (int p = tid + kKvWriteRegs * kKvWriteThreads; p < pieces; p += kKvWriteThreads) {
-    const uint4 v = ld_cg128(x + (p / per) * rs + (p % per) * 8);
+    const uint4 v = ld_cg128(x + (p / kPer) * rs + (p % kPer) * 8);
     m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(m, v.x), v.y), v.z), v.w);
   }
   m = max(m & 0xFFFFu, m >> 16);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((tid & 31) == 0) red[tid >> 5] = m;
-  const bool older = t0 > begin;
-  const float was = older ? *scale_p : 0.f;
   __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
   for (int w = 0; w < kKvWriteThreads / 32; ++w) m = max(m, red[w]);
@@ -149,16 +170,16 @@ __global__ void __launch_bounds__(kKvWriteThreads) kv_write_kernel(const KvWrite
 
   if (older && scale != was) {
     const float ratio = scale > 0.f ? __fdiv_rn(was, scale) : 0.f;
-    const int old_pieces = (t0 - begin) * a.c.D >> 4;
+    const int old_pieces = (t0 - begin) * kD >> 4;
     uint4* o = reinterpret_cast<uint4*>(codes);
     for (int p = tid; p < old_pieces; p += kKvWriteThreads) {
-      uint4 v = o[p];
+      uint4 v = ld_cg128(o + p);
       v.x = kv_rescale4(v.x, ratio), v.y = kv_rescale4(v.y, ratio);
       v.z = kv_rescale4(v.z, ratio), v.w = kv_rescale4(v.w, ratio);
       o[p] = v;
     }
   }
-  uint2* o = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(t0 - begin) * a.c.D);
+  uint2* o = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(t0 - begin) * kD);
   auto put = [&](int p, uint4 v) {
     o[p] = make_uint2(kv_codes4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y), inv),
                       kv_codes4(bf16_lo(v.z), bf16_hi(v.z), bf16_lo(v.w), bf16_hi(v.w), inv));
@@ -167,7 +188,7 @@ __global__ void __launch_bounds__(kKvWriteThreads) kv_write_kernel(const KvWrite
   for (int j = 0; j < kKvWriteRegs; ++j)
     if (tid + j * kKvWriteThreads < pieces) put(tid + j * kKvWriteThreads, keep[j]);
   for (int p = tid + kKvWriteRegs * kKvWriteThreads; p < pieces; p += kKvWriteThreads)
-    put(p, ld_cg128(x + (p / per) * rs + (p % per) * 8));
+    put(p, ld_cg128(x + (p / kPer) * rs + (p % kPer) * 8));
 }
 
 struct KvReadArgs {
@@ -188,35 +209,53 @@ __device__ __forceinline__ uint2 kv_values4(uint32_t w, float s) {
   return make_uint2(pack_bf16x2(f(0x7440), f(0x7441)), pack_bf16x2(f(0x7442), f(0x7443)));
 }
 
-// Row i of the output is position len - rows + i (0 where that is negative).  One thread moves 16 codes.
+// Row i of the output is position len - rows + i (0 where that is negative).  A thread moves kKvReadPieces times 16 codes,
+// with all its table entries, then all its codes on their way at once, and stores 32 bytes at a time: 16-byte stores at
+// 32-byte steps cost a third more (15k tokens of 8 heads of 128: 25 us).  blockIdx = (pieces, K or V, sequence).
+constexpr int kKvReadPieces = 2;
+template <int kD>
 __global__ void __launch_bounds__(kKvReadThreads) kv_read_kernel(const KvReadArgs a) {
+  constexpr int kPer = kD / 16, kN = kKvReadPieces;
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.y, which = blockIdx.z;
-  const int per = a.c.D >> 4;
-  const int64_t p = static_cast<int64_t>(blockIdx.x) * kKvReadThreads + threadIdx.x;
-  const int64_t all = static_cast<int64_t>(a.rows) * a.c.kv_heads * per;
-  if (p >= all) return;
-  const int d = static_cast<int>(p % per);
-  const int64_t rh = p / per;
-  const int h = static_cast<int>(rh % a.c.kv_heads), r = static_cast<int>(rh / a.c.kv_heads);
-  const int pos = ld_cg(a.lens + b) - a.rows + r;
-  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  if (pos >= 0) {
-    const int64_t page = kv_page(a.c, b, pos >> a.c.log2_page);
-    if (page >= 0) {
-      const int64_t at = page * a.c.kv_heads + h;
-      const float s = ld_cg(a.scales[which] + at);
-      const int in = pos & ((1 << a.c.log2_page) - 1);
-      const uint4 w = ld_cg128(a.codes[which] + ((at << a.c.log2_page) + in) * a.c.D + d * 16);
-      const uint2 v0 = kv_values4(w.x, s), v1 = kv_values4(w.y, s), v2 = kv_values4(w.z, s), v3 = kv_values4(w.w, s);
-      lo = make_uint4(v0.x, v0.y, v1.x, v1.y);
-      hi = make_uint4(v2.x, v2.y, v3.x, v3.y);
-    }
+  const int b = blockIdx.z, which = blockIdx.y, lg = a.c.log2_page;
+  const uint32_t all = static_cast<uint32_t>(a.rows) * a.c.kv_heads * kPer;  // fits: checked on the host
+  const uint32_t p0 = blockIdx.x * (kKvReadThreads * kN) + threadIdx.x;
+  const int begin = ld_cg(a.lens + b) - a.rows;
+  const int32_t* table = a.c.table + static_cast<int64_t>(b) * a.c.table_cols;
+  const int8_t* codes = which ? a.codes[1] : a.codes[0];
+  const float* scales = which ? a.scales[1] : a.scales[0];
+  bf16* out = which ? a.y[1] : a.y[0];
+  uint32_t entry[kN];
+  int pos[kN], h[kN];
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const uint32_t rh = (p0 + j * kKvReadThreads) / kPer, r = rh / a.c.kv_heads;
+    h[j] = rh - r * a.c.kv_heads;
+    pos[j] = p0 + j * kKvReadThreads < all ? begin + static_cast<int>(r) : -1;
+    entry[j] = 0xFFFFFFFFu;
+    ld_cg32_if(entry[j], table + (pos[j] >> lg), pos[j] >= 0 && (pos[j] >> lg) < a.c.table_cols);
   }
-  uint4* y = reinterpret_cast<uint4*>(a.y[which] + static_cast<int64_t>(b) * all * 16 + p * 16);
-  y[0] = lo;
-  y[1] = hi;
+  uint4 w[kN];
+  uint32_t s[kN];
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const bool on = pos[j] >= 0 && kv_page_ok(a.c, static_cast<int>(entry[j]));
+    const int64_t at = static_cast<int64_t>(on ? entry[j] : 0u) * a.c.kv_heads + h[j];
+    w[j] = make_uint4(0, 0, 0, 0);
+    s[j] = 0;
+    ld_cg32_if(s[j], scales + at, on);
+    ld_cg128_if(w[j], codes + ((at << lg) + (pos[j] & ((1 << lg) - 1))) * kD + (p0 + j * kKvReadThreads) % kPer * 16, on);
+  }
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const uint32_t p = p0 + j * kKvReadThreads;
+    if (p >= all) break;
+    const float sc = __uint_as_float(s[j]);
+    const uint2 v0 = kv_values4(w[j].x, sc), v1 = kv_values4(w[j].y, sc), v2 = kv_values4(w[j].z, sc), v3 = kv_values4(w[j].w, sc);
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + (static_cast<int64_t>(b) * all + p) * 16),
+                 "r"(v0.x), "r"(v0.y), "r"(v1.x), "r"(v1.y), "r"(v2.x), "r"(v2.y), "r"(v3.x), "r"(v3.y) : "memory");
+  }
 }
 
 }  // namespace gguf_b200

@@ -328,7 +328,7 @@ GGUF_OPS_API int gguf_kv_cache_write(const GgufKvCache* cache, const void* k, co
 
 /*
  * KvCacheRead: the last `rows` tokens of every sequence as bf16(code * scale), k and v [B, rows, kv_heads, head_dim];
- * row i is position lens[b] - rows + i, zeros where that is negative.
+ * row i is position lens[b] - rows + i, zeros where that is negative.  k and v 32-byte aligned.
  */
 GGUF_OPS_API int gguf_kv_cache_read(const GgufKvCache* cache, const int32_t* table, const int32_t* lens, void* k, void* v,
                                     int64_t B, int64_t rows, int64_t table_cols, void* stream);
