@@ -54,6 +54,11 @@ def _stream(stream=None) -> int:
     return s.cuda_stream
 
 
+def _raw_stream(t: torch.Tensor) -> int:
+    """The current stream of t's device as the C ABI takes it (a stream object costs 3 us of host time a call)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -489,9 +494,11 @@ def MambaVerifyGGUF(proj, conv_state, ssm_state, conv_w, conv_b, dt_bias, A_neg,
 # ------------------------------------------------------------------------------------------------
 def qk_norm_rope_into(x, q_gamma, k_gamma, cos, sin, positions, q, k, T: int, row_stride: int, heads: int, kv_heads: int,
                       head_dim: int, rot: int, max_pos: int, eps: float, interleaved: int, stream=None) -> None:
-    check(load().gguf_qk_norm_rope(_ptr(x), _ptr(q_gamma), _ptr(k_gamma), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(q),
-                                   _ptr(k), T, row_stride, heads, kv_heads, head_dim, rot, max_pos, eps, interleaved,
-                                   _stream(stream)))
+    rc = load().gguf_qk_norm_rope(x.data_ptr(), _ptr(q_gamma), _ptr(k_gamma), cos.data_ptr(), sin.data_ptr(),
+                                  positions.data_ptr(), q.data_ptr(), k.data_ptr(), T, row_stride, heads, kv_heads, head_dim, rot,
+                                  max_pos, eps, interleaved, _raw_stream(x) if stream is None else stream.cuda_stream)
+    if rc:
+        check(rc)
 
 
 def QkNormRope(qkv: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None, cos: torch.Tensor,
@@ -529,8 +536,8 @@ def QkNormRope(qkv: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.T
             if t.numel() != D:
                 raise ValueError(f"QkNormRope: {n} size mismatch")
     lead = qkv.shape[:-1]
-    q = torch.empty(*lead, heads, D, dtype=torch.bfloat16, device=qkv.device)
-    k = torch.empty(*lead, kv_heads, D, dtype=torch.bfloat16, device=qkv.device)
+    q = qkv.new_empty((*lead, heads, D))
+    k = qkv.new_empty((*lead, kv_heads, D))
     qk_norm_rope_into(qkv2, q_gamma, k_gamma, cos, sin, positions, q, k, T, qkv2.stride(0), heads, kv_heads, D,
                       2 * cos.shape[1], cos.shape[0], epsilon, 1 if interleaved else 0)
     return q, k
@@ -597,8 +604,10 @@ def _kv_rows(op, name, t, B, heads, D):
 
 def kv_cache_write_into(cache: KvCache, k, v, page_table, lens, new_lens, B: int, R: int, cols: int, k_strides, v_strides,
                         stream=None) -> None:
-    check(load().gguf_kv_cache_write(cache._ref, _ptr(k), _ptr(v), _ptr(page_table), _ptr(lens), _ptr(new_lens), B, R, cols,
-                                     *k_strides, *v_strides, _stream(stream)))
+    rc = load().gguf_kv_cache_write(cache._ref, k.data_ptr(), v.data_ptr(), page_table.data_ptr(), lens.data_ptr(), _ptr(new_lens),
+                                    B, R, cols, *k_strides, *v_strides, _raw_stream(k) if stream is None else stream.cuda_stream)
+    if rc:
+        check(rc)
 
 
 def KvCacheWrite(k: torch.Tensor, v: torch.Tensor, cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor,
@@ -618,8 +627,10 @@ def KvCacheWrite(k: torch.Tensor, v: torch.Tensor, cache: KvCache, page_table: t
 
 
 def kv_cache_read_into(cache: KvCache, page_table, lens, k, v, B: int, rows: int, cols: int, stream=None) -> None:
-    check(load().gguf_kv_cache_read(cache._ref, _ptr(page_table), _ptr(lens), _ptr(k), _ptr(v), B, rows, cols,
-                                    _stream(stream)))
+    rc = load().gguf_kv_cache_read(cache._ref, page_table.data_ptr(), lens.data_ptr(), k.data_ptr(), v.data_ptr(), B, rows, cols,
+                                   _raw_stream(k) if stream is None else stream.cuda_stream)
+    if rc:
+        check(rc)
 
 
 def KvCacheRead(cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor, *, rows: int):
@@ -678,9 +689,12 @@ def _kv_workspace(device, stream) -> KvAttentionWorkspace:
 def kv_cache_attention_into(cache: KvCache, q, page_table, lens, new_lens, out, lse, workspace: KvAttentionWorkspace,
                             B: int, R: int, heads: int, cols: int, q_strides, scale: float, window: int,
                             stream=None) -> None:
-    check(load().gguf_kv_cache_attention(cache._ref, _ptr(q), _ptr(page_table), _ptr(lens), _ptr(new_lens), _ptr(out),
-                                         _ptr(lse), _ptr(workspace.scratch), _ptr(workspace.counters), B, R, heads, cols,
-                                         *q_strides, scale, window, _stream(stream)))
+    rc = load().gguf_kv_cache_attention(cache._ref, q.data_ptr(), page_table.data_ptr(), lens.data_ptr(), _ptr(new_lens),
+                                        out.data_ptr(), _ptr(lse), workspace.scratch.data_ptr(), workspace.counters.data_ptr(), B, R,
+                                        heads, cols, *q_strides, scale, window,
+                                        _raw_stream(q) if stream is None else stream.cuda_stream)
+    if rc:
+        check(rc)
 
 
 def KvCacheAttention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor,
@@ -699,20 +713,22 @@ def KvCacheAttention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, 
     R, heads = q.shape[1], q.shape[2]
     if heads == 0 or heads % cache.kv_heads != 0:
         raise ValueError(f"{op}: heads must be a multiple of kv heads")
-    out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(B, R, heads, dtype=torch.float32, device=q.device) if return_lse else None
-    stream = torch.cuda.current_stream()
-    ws = workspace if workspace is not None else _kv_workspace(q.device, stream.cuda_stream)
+    ws = workspace if workspace is not None else _kv_workspace(q.device, _raw_stream(q))
     ws.fit(B, R, heads, cache.kv_heads, cache.head_dim)
     kv_cache_attention_into(cache, q, page_table, lens, new_lens, out, lse, ws, B, R, heads, cols, strides,
-                            cache.head_dim ** -0.5 if scale is None else scale, window, stream)
+                            cache.head_dim ** -0.5 if scale is None else scale, window)
     return (out, lse) if return_lse else out
 
 
 def draft_verify_into(target, draft_probs, draft, u_accept, u_sample, drafts, accepted, tokens, B: int, R: int, V: int,
                       stream=None) -> None:
-    check(load().gguf_draft_verify(_ptr(target), _ptr(draft_probs), _ptr(draft), _ptr(u_accept), _ptr(u_sample),
-                                   _ptr(drafts), _ptr(accepted), _ptr(tokens), B, R, V, _stream(stream)))
+    rc = load().gguf_draft_verify(target.data_ptr(), _ptr(draft_probs), draft.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(),
+                                  _ptr(drafts), accepted.data_ptr(), tokens.data_ptr(), B, R, V,
+                                  _raw_stream(target) if stream is None else stream.cuda_stream)
+    if rc:
+        check(rc)
 
 
 def DraftVerify(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, draft_tokens: torch.Tensor,
@@ -744,8 +760,8 @@ def DraftVerify(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, dr
         _need(drafts, "drafts", torch.int32, op)
         if drafts.shape != (B,):
             raise ValueError(f"{op}: drafts must have one number per sequence")
-    accepted = torch.empty(B, dtype=torch.int32, device=draft_tokens.device)
-    tokens = torch.empty(B, R + 1, dtype=torch.int32, device=draft_tokens.device)
+    accepted = draft_tokens.new_empty((B,))
+    tokens = draft_tokens.new_empty((B, R + 1))
     draft_verify_into(target_probs, draft_probs, draft_tokens, u_accept, u_sample, drafts, accepted, tokens, B, R, V)
     return accepted, tokens
 
