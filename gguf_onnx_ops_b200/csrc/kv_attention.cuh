@@ -141,7 +141,9 @@ struct KvAttnPlan {
   static constexpr int kOBytes = kKvWarps * kFrags * 32 * 16;
   static constexpr int kRowBytes = kRows * (4 + 4 + 4) + kKvWarps * kRows * 8;
   static constexpr int smem(int B) { return kQBytes + kOBytes + kRowBytes + 64 + (B + 1) * 4; }
-  static constexpr int kCtas = kD == 64 ? (kNT == 1 ? 3 : 2) : kD <= 128 ? 2 : 1;  // registers leave room for these
+  // CTAs per SM: two where 128 registers a thread are enough (96 values and 16 rows do not fit: one sequence of 131071
+  // tokens 106 us with two, 81 with one; three for 64 values and 8 rows spill: 44.7 us against 40.9).
+  static constexpr int kCtas = kD > 128 || (kD == 96 && kNT == 2) ? 1 : 2;
 };
 
 template <int kD, int kNT>

@@ -51,7 +51,7 @@ struct KvTilePlan {
   static constexpr int kRaw = kTileStep * kD;            // bytes of a staged step of codes
   static constexpr int kRing = kD == 128 ? 6 : 12;       // staged steps, K and V in turn: 48 KB
   static constexpr int kVAt = kTileBufs * kOperand, kQAt = 2 * kVAt, kRingAt = kQAt + 2 * kQTile, kCtrlAt = kRingAt + kRing * kRaw;
-  static constexpr int kCtrl = 4080;                     // scales, barriers, small shared state
+  static constexpr int kCtrl = 6128;                     // scales, barriers, small shared state
   static constexpr int smem(int B) { return 1024 + kCtrlAt + kCtrl + (B + 1) * 4; }
   // Tensor memory columns of stream s: its two S (the f16 weights over their S), O.
   __host__ __device__ static constexpr uint32_t s_at(int s, int buf) { return 128u * s + 64u * buf; }
@@ -66,9 +66,9 @@ struct KvTileCtrl {
   uint32_t tmem;
   int scan[28];
   float2 hand[kTileRows];   // maximum and sum of stream 1, handed to stream 0
-  float swap[2][2][kTileRows];  // [stream][half][row]: what a row's two threads tell each other
+  float swap[2][2][2][kTileRows];  // [item % 2][stream][half][row]: what a row's two threads tell each other
 };
-static_assert(sizeof(KvTileCtrl) <= 4080, "control block");
+static_assert(sizeof(KvTileCtrl) <= 6128, "control block");
 
 // The token tiles of the 256-row unit rt of a sequence: t0 .. t1 - 1.
 __device__ __forceinline__ void kv_tile_range(const KvAttnArgs& a, const KvSpan& s, int rt, int& t0, int& t1) {
@@ -411,7 +411,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     // thread per row (two warps), waits and tensor-memory latencies left the exp unit idle for two thirds of the time.
     const int s = warp >> 3, half = warp >> 2 & 1, row = tid & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    float *mine = &ct->swap[s][half][row], *other = &ct->swap[s][half ^ 1][row];
+    // Two places in turn: a thread comes back to one only after a barrier that the other reaches having read it.
+    auto tell = [&](uint32_t turn, float v) {
+      ct->swap[turn & 1][s][half][row] = v;
+      bar_sync(2 + s, 2 * kTileRows);
+      return ct->swap[turn & 1][s][half ^ 1][row];
+    };
     uint32_t steps = 0, done = 0;
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
@@ -445,9 +450,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         for (int i = 0; i < kD / 16; ++i)
           m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(m, w[i].x), w[i].y), w[i].z), w[i].w);
         m = max(m & 0xFFFFu, m >> 16);
-        *mine = __uint_as_float(m);
-        bar_sync(2 + s, 2 * kTileRows);
-        m = max(m, __float_as_uint(*other));
+        m = max(m, __float_as_uint(tell(done + 1, __uint_as_float(m))));
         const int e = m ? min(127, 14 - (static_cast<int>(m >> 7) - 127)) : 0;
         qs = pow2i(-e) * fabsf(a.scale_log2);
         if (u.two || s == 0) {
@@ -499,9 +502,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
           }
         };
         if (whole) largest(std::false_type{}); else largest(std::true_type{});
-        *mine = mx;
-        bar_sync(2 + s, 2 * kTileRows);
-        mx = fmaxf(mx, *other);
+        mx = fmaxf(mx, tell(g, mx));
         if (__any_sync(0xffffffffu, mx > m + kTileGrow)) {  // a row's maximum moves: O and the sum shrink
           const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : ex2(m - mn);
           m = mn;
@@ -548,10 +549,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       }
       steps += 2 * tiles;
       done += items;
-      bar_sync(2 + s, 2 * kTileRows);  // (the last maxima have been read)
-      *mine = l;
-      bar_sync(2 + s, 2 * kTileRows);
-      l += *other;  // (each of the two adds the other's: the same sum)
+      l += tell(done, l);  // (each of the two adds the other's: the same sum)
       tile_wait(&ct->pv_done[s][(done - 1) & 1], (done - 1) >> 1, dead);  // (the item two before is known to be done: S)
       tc_fence_after();
 

@@ -73,19 +73,32 @@ cudaError_t run_rope(const RopeArgs& a, bool interleaved, cudaStream_t s) {
 }
 
 // How a call's rows (query tokens x heads of one kv head) are taken: 8 or 16 at a time by the streaming kernel, or 256 at a
-// time by the tile kernel.
+// time by the tile kernel, when there are many rows and much work: the streaming kernel reads a cache once per 16 rows, the
+// tile kernel costs 20 to 30 us in any case (two launches, a pipeline to fill).  Work is what the streaming kernel's line
+// would hold at most, from the page table's width and the window: lengths are on the device.
+// 16 sequences of 801 to 9001 tokens, 8 kv heads, streaming / tile in us, by rows:
+//   128 values: 16 rows 58 / 85, 24 rows 99 / 87, 48 rows 142 / 91; one sequence of 65001: 32 rows 80 / 95, 48 rows 108 / 96
+//   64 values: 32 rows 61 / 82, 48 rows 85 / 83, 64 rows 110 / 83; one sequence of 65001: 48 rows 60 / 80, 96 rows 105 / 82
+// and of the work, in tiles of the line per SM:
+//   128 values, one sequence: 512 rows, 801 tokens (142) 30 / 38; 128 rows, 6401 tokens (187) 40 / 44; 512 rows, 1601 tokens (230) 43 / 39
+//   64 values, one sequence: 512 rows, 1601 tokens (230) 27 / 31; 2048 rows, 256 tokens (330) 31 / 29; 512 rows, 3201 tokens (400) 38 / 33
+// 8 rows of 128 values taken as 16: 57 -> 84 us (one sequence of 131071 tokens).
 struct AttentionPlan {
   bool tile;
   int rows;            // of a unit
   int64_t row_tiles;   // units per kv head
-  int64_t counters(int64_t B, int64_t kv_heads) const { return tile ? 0 : B * kv_heads * row_tiles; }
 };
-AttentionPlan attention_plan(int64_t B, int64_t rows, int64_t D) {
-  AttentionPlan p;
-  p.tile = rows > 16 && (D == 64 || D == 128) && B <= kTileMaxBatch;
-  p.rows = p.tile ? kTileUnitRows : rows <= 8 ? 8 : 16;
-  p.row_tiles = (rows + p.rows - 1) / p.rows;
-  return p;
+int64_t tile_work(int64_t D, int sms) { return sms * (D == 64 ? 300ll : 200ll); }
+bool tile_rows(int64_t B, int64_t rows, int64_t D) { return ((D == 64 && rows > 48) || (D == 128 && rows > 32)) && B <= kTileMaxBatch; }
+AttentionPlan stream_plan(int64_t rows) {
+  const int unit = rows <= 8 ? 8 : 16;
+  return {false, unit, (rows + unit - 1) / unit};
+}
+AttentionPlan attention_plan(int64_t B, int64_t rows, int64_t D, int64_t kv_heads, int64_t positions, int sms) {
+  const AttentionPlan p = stream_plan(rows);
+  const int64_t per_unit = (positions + kKvTile - 1) / kKvTile + kKvUnitCost;
+  if (!tile_rows(B, rows, D) || B * kv_heads * p.row_tiles < tile_work(D, sms) / per_unit) return p;
+  return {true, kTileUnitRows, (rows + kTileUnitRows - 1) / kTileUnitRows};
 }
 
 template <typename Kernel>
@@ -263,9 +276,17 @@ int gguf_kv_cache_attention_workspace(int64_t B, int64_t R, int64_t heads, int64
   if (!known_dim(head_dim)) return invalid(op, "head_dim must be 64, 96, 128, 192 or 256");
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  const AttentionPlan p = attention_plan(B, R * (heads / kv_heads), head_dim);
-  *bytes = attention_dispatch(p, head_dim, [&](auto k) { return k.part_bytes(sms) + k.ml_bytes(sms); });
-  *counters = p.counters(B, kv_heads);
+  auto bytes_of = [&](const AttentionPlan& p) {
+    return attention_dispatch(p, head_dim, [&](auto k) { return k.part_bytes(sms) + k.ml_bytes(sms); });
+  };
+  const int64_t rows = R * (heads / kv_heads);
+  const AttentionPlan p = stream_plan(rows);
+  *bytes = bytes_of(p);
+  *counters = B * kv_heads * p.row_tiles;  // one per unit
+  if (tile_rows(B, rows, head_dim)) {  // either kernel, by the width of the page table; the tile kernel needs no counters
+    *bytes = std::max(*bytes, bytes_of({true, kTileUnitRows, 1}));
+    *counters = std::min(*counters, tile_work(head_dim, sms));
+  }
   return GGUF_OK;
 }
 
@@ -287,7 +308,8 @@ int gguf_kv_cache_attention(const GgufKvCache* cache, const void* q, const int32
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   const int64_t group = heads / cache->kv_heads, rows = R * group;
-  const AttentionPlan p = attention_plan(B, rows, cache->head_dim);
+  const int64_t width = table_cols << a.c.log2_page, positions = window > 0 ? std::min(width, window + R) : width;
+  const AttentionPlan p = attention_plan(B, rows, cache->head_dim, cache->kv_heads, positions, sms);
   if (B * cache->kv_heads * p.row_tiles >= (1ll << 31)) return invalid(op, "too many rows");
   a.k = static_cast<const int8_t*>(cache->k), a.v = static_cast<const int8_t*>(cache->v);
   a.ks = cache->k_scale, a.vs = cache->v_scale;

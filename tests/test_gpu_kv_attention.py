@@ -11,6 +11,7 @@ from gguf_onnx_ops_b200 import ops
 from tests import kv_ref as K
 
 pytestmark = pytest.mark.gpu
+WIDE = 1 << 20  # positions of a wide table, over all (sequence, kv head) pairs
 
 
 def check(out, ref, mag, cache, lens):
@@ -34,15 +35,18 @@ def run_case(cuda, B, R, H, Hk, page, D, lens, news=None, window=0, scale=None, 
         q = (torch.randn(B, R, H, D, generator=K.gen(seed + 2)) * qmul).to(torch.bfloat16).to(cuda)
     lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
     nt = None if news is None else torch.tensor(news, dtype=torch.int32, device=cuda)
-    out, lse = ops.KvCacheAttention(q, ops.KvCache(*cache_t), table, lt, nt, window=window, scale=scale, return_lse=True)
     ref, mag, ref_lse = K.attention(q, cache_t, table, lens, news, D ** -0.5 if scale is None else scale, window)
-    check(out, ref, mag, cache_t, lens)
     seen = torch.isfinite(ref_lse)
-    assert torch.equal(seen, torch.isfinite(lse))
-    assert ((lse.double() - ref_lse)[seen].abs() <= 1e-5 * (4 + ref_lse[seen].abs())).all()
-    assert (out[~seen] == 0).all()
-    again = ops.KvCacheAttention(q, ops.KvCache(*cache_t), table, lt, nt, window=window, scale=scale)
-    assert torch.equal(out, again)  # whatever the order in which CTAs finish
+    # A page table that is much wider than the lengths: for many rows another kernel takes the call.
+    wide = torch.nn.functional.pad(table, (0, WIDE // (B * Hk * page)), value=-1)
+    for t in (table, wide):
+        out, lse = ops.KvCacheAttention(q, ops.KvCache(*cache_t), t, lt, nt, window=window, scale=scale, return_lse=True)
+        check(out, ref, mag, cache_t, lens)
+        assert torch.equal(seen, torch.isfinite(lse))
+        assert ((lse.double() - ref_lse)[seen].abs() <= 1e-5 * (4 + ref_lse[seen].abs())).all()
+        assert (out[~seen] == 0).all()
+        again = ops.KvCacheAttention(q, ops.KvCache(*cache_t), t, lt, nt, window=window, scale=scale)
+        assert torch.equal(out, again)  # whatever the order in which CTAs finish
     return out
 
 
@@ -70,10 +74,18 @@ def test_windows(cuda, window):
     run_case(cuda, 2, 40, 10, 2, 16, 64, [40, 399], window=window, seed=window % 97)
 
 
+@pytest.mark.parametrize("window", [1, 5, 16, 100, 1000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_windows_of_many_rows(cuda, window, D):
+    run_case(cuda, 8, 200, 10, 2, 16, D, [200, 201, 215, 300, 399, 777, 1210, 260], window=window, seed=window,
+             news=[200, 200, 200, 1, 200, 130, 200, 0])
+
+
 @pytest.mark.parametrize("R", [17, 33, 64, 129, 300])
 def test_many_rows(cuda, R):
     run_case(cuda, 2, R, 6, 2, 64, 128, [R, R + 211], seed=R)
     run_case(cuda, 1, R, 3, 1, 16, 64, [R + 1], seed=R)
+    run_case(cuda, 3, R, 4, 2, 256, 64, [R, R + 3, 900], seed=R, news=[R, 3, R // 2])
 
 
 def test_one_long_sequence(cuda):
@@ -136,14 +148,25 @@ def test_hidden_places_do_not_matter(cuda):
 
     run_case(cuda, 1, 1, 8, 2, 32, 128, [161], window=97, seed=12, edit=front)
     run_case(cuda, 1, 20, 8, 2, 32, 128, [161 + 19], window=97, seed=12, edit=front)
+    # the same for many rows
+    run_case(cuda, 1, 20, 8, 2, 32, 128, [101], seed=11, edit=edit)
+
+    def fronts(c, table):
+        for t in c[2:]:
+            t[table[:, :2].long()] = float("inf")
+
+    run_case(cuda, 16, 100, 8, 2, 32, 128, [260 - 100 // (b + 1) % 3 for b in range(16)], window=97, seed=12,
+             news=[100 - 100 // (b + 1) % 3 for b in range(16)], edit=fronts)
 
 
-def test_marked_pages_are_seen(cuda):
+@pytest.mark.parametrize("R,D,cols", [(1, 64, 3), (20, 128, 8000)])
+def test_marked_pages_are_seen(cuda, R, D, cols):
     """A page whose scale is NaN makes the rows that see it NaN, and no others."""
-    c = K.make_cache(8, 2, 16, 64, 1, cuda)
-    table = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device=cuda)
+    c = K.make_cache(8, 2, 16, D, 1, cuda)
+    table = torch.full((2, cols), -1, dtype=torch.int32, device=cuda)
+    table[:, :3] = torch.arange(6, dtype=torch.int32, device=cuda).view(2, 3)
     c[3][4, 1] = float("nan")
-    q = torch.randn(2, 1, 4, 64, generator=K.gen(2)).to(torch.bfloat16).to(cuda)
+    q = torch.randn(2, R, 4, D, generator=K.gen(2)).to(torch.bfloat16).to(cuda)
     lens = torch.tensor([40, 40], dtype=torch.int32, device=cuda)
     out = ops.KvCacheAttention(q, ops.KvCache(*c), table, lens)
     assert torch.isfinite(out[0].float()).all() and torch.isfinite(out[1, :, :2].float()).all()
@@ -166,11 +189,12 @@ def test_strided_queries_streams_and_workspaces(cuda):
     assert torch.equal(a, c)
 
 
-def test_captured_graph_serves_other_lengths(cuda):
-    B, R, H, Hk, page, D = 4, 2, 8, 2, 64, 128
+@pytest.mark.parametrize("R,extra", [(2, 0), (12, 4000)])
+def test_captured_graph_serves_other_lengths(cuda, R, extra):
+    B, H, Hk, page, D = 4, 8, 2, 64, 128
     c = K.make_cache(200, Hk, page, D, 14, cuda)
     cache = ops.KvCache(*c)
-    table = K.make_table(B, 40, 200, 15, cuda)
+    table = torch.nn.functional.pad(K.make_table(B, 40, 200, 15, cuda), (0, extra), value=-1)
     q = torch.randn(B, R, H, D, generator=K.gen(16)).to(torch.bfloat16).to(cuda)
     lens = torch.tensor([5, 100, 900, 2000], dtype=torch.int32, device=cuda)
     ws = ops.KvAttentionWorkspace(cuda)
