@@ -66,7 +66,7 @@ struct KvTileCtrl {
   uint32_t tmem;
   int scan[28];
   float2 hand[kTileRows];   // maximum and sum of stream 1, handed to stream 0
-  float swap[2][2][2][kTileRows];  // [item % 2][stream][half][row]: what a row's two threads tell each other
+  float swap[2][2][2][kTileRows];  // [maxima of items, else][stream][half][row]: what a row's two threads tell each other
 };
 static_assert(sizeof(KvTileCtrl) <= 6128, "control block");
 
@@ -84,12 +84,30 @@ __device__ __forceinline__ void kv_tile_range(const KvAttnArgs& a, const KvSpan&
   t1 = (hi + kTileTokens - 1) / kTileTokens;
 }
 
+__device__ __forceinline__ int kv_tile_cost(const KvAttnArgs& a, const KvSpan& s, int rt) {
+  int t0, t1;
+  kv_tile_range(a, s, rt, t0, t1);
+  return kTileUnitCost + max(1, t1 - t0);
+}
+// Of row tiles 0 .. n - 1, by a whole warp (one thread takes 5500 cycles for 16 row tiles).
+__device__ __forceinline__ int kv_tile_cost_sum(const KvAttnArgs& a, const KvSpan& s, int n) {
+  int c = 0;
+  for (int rt = threadIdx.x & 31; rt < n; rt += 32) c += kv_tile_cost(a, s, rt);
+  return __reduce_add_sync(0xffffffffu, c);
+}
+// 32-bit where the numbers allow it: a 64-bit division is some hundred instructions.
+__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 struct KvTileUnit {
   KvSpan sp;
   int b, h, rt, t0, ta, tb, tiles;  // token tiles t0 + ta .. t0 + tb - 1 of this CTA, of `tiles`
   int taken;                        // how far the slice has come with it
   bool mine, work, two;             // mine: tiles are this CTA's; work: rows see something; two: two row tiles
 };
+// The unit that holds place `at` of the line (called by whole warps).
 __device__ __forceinline__ KvTileUnit kv_tile_unit(const KvAttnArgs& a, const int* prefix, int64_t at, int64_t end) {
   KvTileUnit u;
   int b = 0;
@@ -101,14 +119,38 @@ __device__ __forceinline__ KvTileUnit kv_tile_unit(const KvAttnArgs& a, const in
   u.sp = kv_span(a, b);
   const int per_head = prefix[b + 1] - prefix[b];
   const int64_t in_seq = at - static_cast<int64_t>(prefix[b]) * a.c.kv_heads;
-  u.h = static_cast<int>(in_seq / per_head);
-  int rem = static_cast<int>(in_seq % per_head), t1 = 0;
-  for (u.rt = 0;; ++u.rt) {
-    kv_tile_range(a, u.sp, u.rt, u.t0, t1);
-    u.tiles = max(1, t1 - u.t0);
-    if (rem < kTileUnitCost + u.tiles || u.rt + 1 >= a.row_tiles) break;
-    rem -= kTileUnitCost + u.tiles;
+  u.h = static_cast<int>(kv_div(in_seq, per_head));
+  int rem = static_cast<int>(in_seq - static_cast<int64_t>(u.h) * per_head), t1 = 0;
+  if (a.row_tiles == 1) {
+    u.rt = 0;
+    kv_tile_range(a, u.sp, 0, u.t0, t1);
+  } else {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0;; base += 32) {
+      const int rt = base + lane;
+      int mt0 = 0, mt1 = 0, cost = 0;
+      if (rt < a.row_tiles) {
+        kv_tile_range(a, u.sp, rt, mt0, mt1);
+        cost = kTileUnitCost + max(1, mt1 - mt0);
+      }
+      int sum = cost;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, rem < sum || rt >= a.row_tiles - 1);
+      if (hit) {
+        const int f = __ffs(hit) - 1;
+        u.rt = base + f;
+        u.t0 = __shfl_sync(0xffffffffu, mt0, f), t1 = __shfl_sync(0xffffffffu, mt1, f);
+        rem -= __shfl_sync(0xffffffffu, sum - cost, f);
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, sum, 31);
+    }
   }
+  u.tiles = max(1, t1 - u.t0);
   u.taken = static_cast<int>(min(static_cast<int64_t>(kTileUnitCost + u.tiles - rem), end - at));
   u.ta = max(0, rem - kTileUnitCost);
   u.tb = rem + u.taken - kTileUnitCost;
@@ -122,17 +164,17 @@ __device__ __forceinline__ KvTileUnit kv_tile_unit(const KvAttnArgs& a, const in
 template <int kThreads>
 __device__ __forceinline__ int kv_tile_prefix(const KvAttnArgs& a, int* prefix, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (a.row_tiles > 1) {
+    for (int b = warp; b < a.B; b += kThreads / 32) {
+      const int c = kv_tile_cost_sum(a, kv_span(a, b), a.row_tiles);
+      if (lane == 0) prefix[b + 1] = c;
+    }
+    __syncthreads();
+  }
   int carry = 0;
   for (int b0 = 0; b0 < a.B; b0 += kThreads) {
     int n = 0;
-    if (b0 + tid < a.B) {
-      const KvSpan s = kv_span(a, b0 + tid);
-      for (int rt = 0; rt < a.row_tiles; ++rt) {
-        int t0, t1;
-        kv_tile_range(a, s, rt, t0, t1);
-        n += kTileUnitCost + max(1, t1 - t0);
-      }
-    }
+    if (b0 + tid < a.B) n = a.row_tiles > 1 ? prefix[b0 + tid + 1] : kv_tile_cost(a, kv_span(a, b0 + tid), 0);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, n, o);
@@ -157,12 +199,40 @@ __device__ __forceinline__ int64_t kv_tile_ctas(int64_t total, int grid) {
 // Workspace slot of CTA c's piece of stream s: every CTA cuts at most one unit at its front and one at its end.
 __device__ __forceinline__ int64_t kv_tile_slot(int64_t c, bool begins, int s) { return (2 * c + (begins ? 1 : 0)) * 2 + s; }
 
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // A wait that gives up for good after its first timeout (which is recorded).
 __device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t phase, bool& dead) {
   if (!dead && !mbar_wait(bar, phase & 1u, kSiteTileWait)) dead = true;
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// The same, and whether any of the threads says so.
+__device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
+  uint32_t any;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n bar.red.or.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(any) : "r"(id), "r"(threads), "r"(mine ? 1u : 0u) : "memory");
+  return any != 0;
 }
 
 template <int kD>
@@ -183,8 +253,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         mbar_init(&ct->k_empty[i], 2), mbar_init(&ct->v_empty[i], 2);
       }
       for (int i = 0; i < 2; ++i) {
-        for (int j = 0; j < 2; ++j) mbar_init(&ct->s_full[i][j], 1), mbar_init(&ct->p_full[i][j], 2 * kTileRows), mbar_init(&ct->pv_done[i][j], 1);
-        mbar_init(&ct->q_full[i], 2 * kTileRows);
+        for (int j = 0; j < 2; ++j) mbar_init(&ct->s_full[i][j], 1), mbar_init(&ct->p_full[i][j], 8), mbar_init(&ct->pv_done[i][j], 1);
+        mbar_init(&ct->q_full[i], 8);
       }
       for (int i = 0; i < P::kRing; ++i) mbar_init(&ct->raw_full[i], 1), mbar_init(&ct->raw_empty[i], kTileConvertWarps / 2);
       fence_mbar_init();
@@ -198,8 +268,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
   tc_fence_after();
   // All 512 columns are this CTA's, so they begin at column 0 (KvTilePlan has their use).
   const int64_t total = static_cast<int64_t>(carry) * a.c.kv_heads, ctas = kv_tile_ctas(total, gridDim.x);
-  const int64_t from = total * blockIdx.x / max(ctas, static_cast<int64_t>(1));
-  const int64_t end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : from;
+  const int64_t from = kv_div(total * blockIdx.x, max(ctas, static_cast<int64_t>(1)));
+  const int64_t end = blockIdx.x < ctas ? kv_div(total * (blockIdx.x + 1), ctas) : from;
   bool dead = false;
 
   if (warp >= kTileConvertWarp && warp < kTileMmaWarp) {
@@ -411,11 +481,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     // thread per row (two warps), waits and tensor-memory latencies left the exp unit idle for two thirds of the time.
     const int s = warp >> 3, half = warp >> 2 & 1, row = tid & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    // Two places in turn: a thread comes back to one only after a barrier that the other reaches having read it.
-    auto tell = [&](uint32_t turn, float v) {
-      ct->swap[turn & 1][s][half][row] = v;
-      bar_sync(2 + s, 2 * kTileRows);
-      return ct->swap[turn & 1][s][half ^ 1][row];
+    // The two threads of a row are in warps w and w + 4 of the stream; a barrier of those two (64 threads) is enough.
+    const int pair = 2 + s * 4 + (warp & 3);
+    auto tell = [&](int place, float v) {  // place 1: maxima of items; 0: the end's sums, before that the rows' scales
+      ct->swap[place][s][half][row] = v;
+      bar_sync(pair, 64);
+      return ct->swap[place][s][half ^ 1][row];
     };
     uint32_t steps = 0, done = 0;
     for (int64_t at = from; at < end;) {
@@ -438,34 +509,43 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       const int base = (u.t0 + u.ta) * kTileTokens + half * 32, hi = u.sp.len - u.sp.n + r + 1;
       const int first = on && a.window > 0 ? max(0, hi - a.window) - base : -base, last = (on ? hi : u.sp.len) - base;
       const int all_first = __reduce_max_sync(0xffffffffu, first), all_last = __reduce_min_sync(0xffffffffu, last);
+      // A warp takes 16 of the stream's rows, kD / 8 lanes a row, so that its loads are whole lines (a row to a thread: 9000
+      // cycles); lane j knows where row j is.
       float qs;
       {
-        const uint4* qr = reinterpret_cast<const uint4*>(a.q + u.b * a.q_stride_b + r * a.q_stride_r +
-                                                         static_cast<int64_t>(u.h * a.group + rr % a.group) * kD) + half * (kD / 16);
-        uint32_t m = 0;
-        uint4 w[kD / 16];
+        constexpr int kLanes = kD / 8, kAtOnce = 32 / kLanes, kLoads = 16 / kAtOnce;
+        const int row0 = (warp & 7) * 16, c = lane % kLanes, tile_at = u.rt * kTileUnitRows + (u.two ? s : 0) * kTileRows;
+        const int my = tile_at + row0 + (lane & 15), my_r = my / a.group;
+        const int64_t my_at = u.b * a.q_stride_b + my_r * a.q_stride_r + static_cast<int64_t>(u.h * a.group + my - my_r * a.group) * kD;
+        const uint32_t rows_on = __ballot_sync(0xffffffffu, my_r < u.sp.n);
+        uint4 w[kLoads];
 #pragma unroll
-        for (int i = 0; i < kD / 16; ++i) w[i] = on ? ld_cg128(qr + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kLoads; ++i) {
+          const int j = i * kAtOnce + lane / kLanes;
+          const int64_t row_at = __shfl_sync(0xffffffffu, my_at, j);
+          w[i] = make_uint4(0, 0, 0, 0);
+          ld_cg128_if(w[i], a.q + row_at + c * 8, rows_on >> j & 1);
+        }
 #pragma unroll
-        for (int i = 0; i < kD / 16; ++i)
-          m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(m, w[i].x), w[i].y), w[i].z), w[i].w);
-        m = max(m & 0xFFFFu, m >> 16);
-        m = max(m, __float_as_uint(tell(done + 1, __uint_as_float(m))));
-        const int e = m ? min(127, 14 - (static_cast<int>(m >> 7) - 127)) : 0;
-        qs = pow2i(-e) * fabsf(a.scale_log2);
-        if (u.two || s == 0) {
-          const float up = a.scale_log2 < 0.f ? -pow2i(e) : pow2i(e);
-          uint8_t* dst = q_buf + s * P::kQTile + row * 128;
+        for (int i = 0; i < kLoads; ++i) {
+          const int j = row0 + i * kAtOnce + lane / kLanes;
+          uint32_t m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(0u, w[i].x), w[i].y), w[i].z), w[i].w);
+          m = max(m & 0xFFFFu, m >> 16);
 #pragma unroll
-          for (int i = 0; i < kD / 16; ++i) {
-            const int c = half * (kD / 16) + i;
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (row & 7)) << 4)) =
+          for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const int e = m ? min(127, 14 - (static_cast<int>(m >> 7) - 127)) : 0;
+          if (c == 0) ct->swap[0][s][0][j] = pow2i(-e) * fabsf(a.scale_log2);
+          if (u.two || s == 0) {
+            const float up = a.scale_log2 < 0.f ? -pow2i(e) : pow2i(e);
+            *reinterpret_cast<uint4*>(q_buf + s * P::kQTile + j * 128 + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (j & 7)) << 4)) =
                 make_uint4(pack_f16x2(bf16_lo(w[i].x) * up, bf16_hi(w[i].x) * up), pack_f16x2(bf16_lo(w[i].y) * up, bf16_hi(w[i].y) * up),
                            pack_f16x2(bf16_lo(w[i].z) * up, bf16_hi(w[i].z) * up), pack_f16x2(bf16_lo(w[i].w) * up, bf16_hi(w[i].w) * up));
           }
-          fence_proxy_async_smem();
         }
-        mbar_arrive(&ct->q_full[s]);
+        fence_proxy_async_smem();
+        bar_sync(10 + s, 2 * kTileRows);
+        if (lane == 0) mbar_arrive(&ct->q_full[s]);
+        qs = ct->swap[0][s][0][row];
       }
       const int tiles = u.tb - u.ta, items = u.two ? 2 * tiles : tiles;
       float m = -INFINITY, l = 0.f;
@@ -502,9 +582,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
           }
         };
         if (whole) largest(std::false_type{}); else largest(std::true_type{});
-        mx = fmaxf(mx, tell(g, mx));
-        if (__any_sync(0xffffffffu, mx > m + kTileGrow)) {  // a row's maximum moves: O and the sum shrink
-          const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : ex2(m - mn);
+        if (bar_any(pair, 64, mx > m + kTileGrow)) {  // a row's maximum moves: O and the sum shrink
+          const float mn = fmaxf(m, fmaxf(mx, tell(1, mx))), f = mn == -INFINITY ? 1.f : ex2(m - mn);
           m = mn;
           l *= f;
           if (i > 0) {
@@ -526,30 +605,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         auto weights = [&](auto cut) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float lift = lv[k] - top;
-            float sum[2] = {0.f, 0.f};
+            const uint64_t lift = pack_f32x2(lv[k] - top, lv[k] - top), mul = pack_f32x2(cs[k], cs[k]);
+            uint64_t sum = 0;
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-              float w0 = ex2(fmaf(__uint_as_float(x[16 * k + j]), cs[k], lift)), w1 = ex2(fmaf(__uint_as_float(x[16 * k + j + 1]), cs[k], lift));
+              const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[16 * k + j]), __uint_as_float(x[16 * k + j + 1])), mul, lift));
+              float w0 = ex2(y.x), w1 = ex2(y.y);
               if constexpr (cut) {
                 w0 = bits >> (16 * k + j) & 1 ? w0 : 0.f;
                 w1 = bits >> (16 * k + j + 1) & 1 ? w1 : 0.f;
               }
-              sum[0] += w0, sum[1] += w1;
+              sum = add_f32x2(sum, pack_f32x2(w0, w1));
               w[k * 8 + j / 2] = pack_f16x2(w0, w1);
             }
-            if (!cut || bits >> (16 * k) & 0xFFFFu) l = fmaf(sum[0] + sum[1], iv[k], l);  // (a hidden page's scale may be anything)
+            if (!cut || bits >> (16 * k) & 0xFFFFu) l = fmaf(unpack_f32x2(sum).x + unpack_f32x2(sum).y, iv[k], l);  // (a hidden page's scale may be anything)
           }
         };
         if (whole) weights(std::false_type{}); else weights(std::true_type{});
         tmem_st16(ts + half * 16, w);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&ct->p_full[s][g & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ct->p_full[s][g & 1]);
       }
       steps += 2 * tiles;
       done += items;
-      l += tell(done, l);  // (each of the two adds the other's: the same sum)
+      l += tell(0, l);  // (each of the two adds the other's: the same sum)
       tile_wait(&ct->pv_done[s][(done - 1) & 1], (done - 1) >> 1, dead);  // (the item two before is known to be done: S)
       tc_fence_after();
 
@@ -628,69 +709,98 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
 
 // Joins the pieces that the tile kernel left, in the order of the tokens.  A launch of its own, after the tile kernel: joining
 // inside it, by the CTA that finishes a unit last, took 9 us of its end (fence, counter, then one thread per row reading
-// piece after piece); here every row has eight threads, and the search for the pieces runs before the wait for the tile kernel.
-// blockIdx = (32 rows of a row tile, kv head, sequence); a thread takes a row and kD / 8 of its values.
-constexpr int kJoinThreads = 256;
-template <int kD>
+// piece after piece).  A unit with few rows and many tokens has up to two pieces per CTA of the tile kernel, so the loads of
+// many pieces have to be in flight at once: first the factors of up to kJoinChunk pieces, then the pieces.
+// blockIdx = (kRows rows of a row tile, kv head, sequence); a thread takes one float4 of kD / 4 and every kBase-th row.
+constexpr int kJoinThreads = 256, kJoinChunk = 32;
+template <int kD, int kGroups>
+struct KvJoinPlan {
+  static constexpr int kVecs = kD / 4, kBase = kJoinThreads / kVecs, kRows = kBase * kGroups;
+};
+template <int kD, int kGroups>
 __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const KvAttnArgs a, int grid) {
-  extern __shared__ int join_prefix[];
+  using P = KvJoinPlan<kD, kGroups>;
+  constexpr int kRows = P::kRows, kBase = P::kBase;
+  extern __shared__ int prefix[];
+  __shared__ float factor[kJoinChunk][kRows];
   __shared__ int scan[kJoinThreads / 32];
+  __shared__ float2 part_ml[kJoinThreads / kRows][kRows];
   // (The lengths are older than the tile kernel, which begins only when its own predecessor is done.)
-  const int64_t total = static_cast<int64_t>(kv_tile_prefix<kJoinThreads>(a, join_prefix, scan)) * a.c.kv_heads;
+  const int64_t total = static_cast<int64_t>(kv_tile_prefix<kJoinThreads>(a, prefix, scan)) * a.c.kv_heads;
   const int64_t ctas = kv_tile_ctas(total, grid);
-  const int b = blockIdx.z, h = blockIdx.y, rt = blockIdx.x * 32 / kTileUnitRows, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, b = blockIdx.z, h = blockIdx.y, rr0 = blockIdx.x * kRows, rt = rr0 / kTileUnitRows;
   const KvSpan sp = kv_span(a, b);
-  int t0 = 0, t1 = 0, before = 0;
-  for (int i = 0; i < rt; ++i) {
-    kv_tile_range(a, sp, i, t0, t1);
-    before += kTileUnitCost + max(1, t1 - t0);
-  }
+  int t0 = 0, t1 = 0;
+  const int before = kv_tile_cost_sum(a, sp, rt);
   kv_tile_range(a, sp, rt, t0, t1);
   const int tiles = max(1, t1 - t0);
-  const int64_t begin = static_cast<int64_t>(join_prefix[b]) * a.c.kv_heads + static_cast<int64_t>(join_prefix[b + 1] - join_prefix[b]) * h + before;
+  const int64_t begin = static_cast<int64_t>(prefix[b]) * a.c.kv_heads + static_cast<int64_t>(prefix[b + 1] - prefix[b]) * h + before;
   const int64_t first = begin + kTileUnitCost;  // of the unit's tiles
-  const int64_t c0 = ((first + 1) * ctas - 1) / total, c1 = ((first + tiles) * ctas - 1) / total;
+  const int64_t c0 = kv_div((first + 1) * ctas - 1, total), c1 = kv_div((first + tiles) * ctas - 1, total);
   const bool two = a.R * a.group - rt * kTileUnitRows > kTileRows;
   pdl_wait();
   pdl_launch_dependents();
   if (t1 <= t0 || c0 == c1) return;  // written by the tile kernel
-  const int rr = blockIdx.x * 32 + lane, r = rr / a.group;
-  if (r >= a.R) return;
-  const int row = rr % kTileRows, s0 = two ? rr % kTileUnitRows / kTileRows : 0, streams = two ? 1 : 2;
-  const int pieces = static_cast<int>(c1 - c0 + 1) * streams;
-  auto slot_of = [&](int p) { return kv_tile_slot(c0 + p / streams, p < streams, two ? s0 : p % streams); };
-  const int64_t out_row = (static_cast<int64_t>(b) * a.R + r) * a.heads + h * a.group + rr % a.group;
-  constexpr int kVecs = kD / 32;  // float4 of this thread
-  float4 acc[kVecs];
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int s0 = two ? rr0 % kTileUnitRows / kTileRows : 0, row0 = rr0 % kTileRows;
+  const int pieces = static_cast<int>(c1 - c0 + 1) << (two ? 0 : 1);
+  auto slot_of = [&](int p) { return two ? kv_tile_slot(c0 + p, p == 0, s0) : kv_tile_slot(c0 + (p >> 1), p < 2, p & 1); };
+
+  // Maxima and factors: a thread takes a row and every kEvery-th piece.
+  constexpr int kEvery = kJoinThreads / kRows;
+  const int frow = tid % kRows, q = tid / kRows;
+  const float2* ml0 = a.ml + row0 + frow;
   float m = -INFINITY, l = 0.f;
-  if (r < sp.n) {
 #pragma unroll 4
-    for (int p = 0; p < pieces; ++p) {
-      const float2 ml = ld_cg(a.ml + slot_of(p) * kTileRows + row);
-      m = fmaxf(m, ml.x);
-    }
-#pragma unroll 2
-    for (int p = 0; p < pieces; ++p) {
-      const int64_t slot = slot_of(p);
-      const float2 ml = ld_cg(a.ml + slot * kTileRows + row);
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-      l = fmaf(ml.y, f, l);
+  for (int p = q; p < pieces; p += kEvery) m = fmaxf(m, ld_cg(ml0 + slot_of(p) * kTileRows).x);
+  part_ml[q][frow].x = m;
+  __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const float4 v = ld_cg(a.part + (slot * (kD / 4) + warp * kVecs + i) * kTileRows + row);
-        acc[i].x = fmaf(v.x, f, acc[i].x), acc[i].y = fmaf(v.y, f, acc[i].y);
-        acc[i].z = fmaf(v.z, f, acc[i].z), acc[i].w = fmaf(v.w, f, acc[i].w);
+  for (int i = 0; i < kEvery; ++i) m = fmaxf(m, part_ml[i][frow].x);
+
+  const int c = tid / kBase, sub = tid % kBase;
+  const float4* src = a.part + static_cast<int64_t>(c) * kTileRows + row0 + sub;
+  float4 acc[kGroups];
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < pieces; p0 += kJoinChunk) {
+    const int n = min(kJoinChunk, pieces - p0);
+    __syncthreads();  // (the maxima, or the last factors, have been read)
+#pragma unroll 4
+    for (int p = q; p < n; p += kEvery) {
+      const float2 ml = ld_cg(ml0 + slot_of(p0 + p) * kTileRows);
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+      factor[p][frow] = f;
+      l = fmaf(ml.y, f, l);
+    }
+    __syncthreads();
+#pragma unroll(8 / kGroups)
+    for (int p = 0; p < n; ++p) {
+      const float4* v0 = src + slot_of(p0 + p) * (P::kVecs * kTileRows);
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        const float f = factor[p][sub + j * kBase];
+        const float4 v = ld_cg(v0 + j * kBase);
+        acc[j].x = fmaf(v.x, f, acc[j].x), acc[j].y = fmaf(v.y, f, acc[j].y);
+        acc[j].z = fmaf(v.z, f, acc[j].z), acc[j].w = fmaf(v.w, f, acc[j].w);
       }
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint2* o = reinterpret_cast<uint2*>(a.o + out_row * kD) + warp * kVecs;
+  part_ml[q][frow] = make_float2(m, l);
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i)
-    o[i] = r < sp.n ? make_uint2(pack_bf16x2(acc[i].x * inv, acc[i].y * inv), pack_bf16x2(acc[i].z * inv, acc[i].w * inv)) : make_uint2(0u, 0u);
-  if (a.lse && warp == 0) a.lse[out_row] = l != 0.f ? (m - kTileTop + lg2(l)) * 0.69314718055994531f : -INFINITY;
+  for (int j = 0; j < kGroups; ++j) {
+    const int row = sub + j * kBase, rr = rr0 + row, r = rr / a.group;
+    if (r >= a.R) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEvery; ++i) sum += part_ml[i][row].y;
+    const bool on = r < sp.n;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t out_row = (static_cast<int64_t>(b) * a.R + r) * a.heads + h * a.group + rr % a.group;
+    reinterpret_cast<uint2*>(a.o + out_row * kD)[c] =
+        on ? make_uint2(pack_bf16x2(acc[j].x * inv, acc[j].y * inv), pack_bf16x2(acc[j].z * inv, acc[j].w * inv)) : make_uint2(0u, 0u);
+    if (a.lse && c == 0) a.lse[out_row] = on && sum != 0.f ? (part_ml[0][row].x - kTileTop + lg2(sum)) * 0.69314718055994531f : -INFINITY;
+  }
 }
 
 }  // namespace gguf_b200

@@ -133,6 +133,12 @@ struct Stream {
 template <int kD>
 struct Tile {
   using P = KvTilePlan<kD>;
+  template <int kGroups>
+  static cudaError_t join(const KvAttnArgs& a, int sms, cudaStream_t s) {
+    using J = KvJoinPlan<kD, kGroups>;
+    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.R) * a.group + J::kRows - 1) / J::kRows), static_cast<unsigned>(a.c.kv_heads), static_cast<unsigned>(a.B));
+    return launch_kernel(kv_attention_join_kernel<kD, kGroups>, grid, dim3(kJoinThreads), (a.B + 1) * sizeof(int), s, a, sms);
+  }
   static int64_t part_bytes(int sms) { return 4ll * sms * kTileRows * kD * 4; }
   static int64_t ml_bytes(int sms) { return 4ll * sms * kTileRows * 8; }
   static int run(const KvAttnArgs& a, int sms, cudaStream_t s) {
@@ -148,8 +154,9 @@ struct Tile {
     if (int rc = raise_smem(kv_attention_tile_kernel<kD>, P::smem(kTileMaxBatch), done)) return rc;
     cudaError_t e = launch_kernel(kv_attention_tile_kernel<kD>, dim3(static_cast<unsigned>(sms)), dim3(kTileThreads), P::smem(a.B), s, a);
     if (e != cudaSuccess) return set_cuda_error("KvCacheAttention launch", e);
-    const dim3 rows(static_cast<unsigned>((static_cast<int64_t>(a.R) * a.group + 31) / 32), static_cast<unsigned>(a.c.kv_heads), static_cast<unsigned>(a.B));
-    e = launch_kernel(kv_attention_join_kernel<kD>, rows, dim3(kJoinThreads), (a.B + 1) * sizeof(int), s, a, sms);
+    // The join's blocks: few rows each while that leaves them in one wave (eight an SM), four times as many after that.
+    const int64_t few = (static_cast<int64_t>(a.R) * a.group + KvJoinPlan<kD, 1>::kRows - 1) / KvJoinPlan<kD, 1>::kRows * a.c.kv_heads * a.B;
+    e = few <= 8ll * sms ? join<1>(a, sms, s) : join<4>(a, sms, s);
     return e == cudaSuccess ? GGUF_OK : set_cuda_error("KvCacheAttention launch", e);
   }
 };
