@@ -51,7 +51,7 @@ struct KvTilePlan {
   static constexpr int kRaw = kTileStep * kD;            // bytes of a staged step of codes
   static constexpr int kRing = kD == 128 ? 6 : 12;       // staged steps, K and V in turn: 48 KB
   static constexpr int kVAt = kTileBufs * kOperand, kQAt = 2 * kVAt, kRingAt = kQAt + 2 * kQTile, kCtrlAt = kRingAt + kRing * kRaw;
-  static constexpr int kCtrl = 6128;                     // scales, barriers, small shared state
+  static constexpr int kCtrl = 8176;                     // scales, barriers, small shared state
   static constexpr int smem(int B) { return 1024 + kCtrlAt + kCtrl + (B + 1) * 4; }
   // Tensor memory columns of stream s: its two S (the f16 weights over their S), O.
   __host__ __device__ static constexpr uint32_t s_at(int s, int buf) { return 128u * s + 64u * buf; }
@@ -62,13 +62,14 @@ struct KvTilePlan {
 struct KvTileCtrl {
   alignas(16) float scale_k[8][4], lv[8][4], inv_v[8][4];  // by step % 8 and group of 16 tokens
   uint64_t k_full[kTileBufs], k_empty[kTileBufs], v_full[kTileBufs], v_empty[kTileBufs], raw_full[12], raw_empty[12];
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full[2];  // [stream][item % 2]: an item is a stream's step
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full[2], q_free;  // [stream][item % 2]: an item is a stream's step
   uint32_t tmem;
   int scan[28];
   float2 hand[kTileRows];   // maximum and sum of stream 1, handed to stream 0
   float swap[2][2][2][kTileRows];  // [maxima of items, else][stream][half][row]: what a row's two threads tell each other
+  float row_scale[2][2][kTileRows];  // [unit % 2][row tile][row]: of the scores
 };
-static_assert(sizeof(KvTileCtrl) <= 6128, "control block");
+static_assert(sizeof(KvTileCtrl) <= 8176, "control block");
 
 // The token tiles of the 256-row unit rt of a sequence: t0 .. t1 - 1.
 __device__ __forceinline__ void kv_tile_range(const KvAttnArgs& a, const KvSpan& s, int rt, int& t0, int& t1) {
@@ -254,8 +255,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       }
       for (int i = 0; i < 2; ++i) {
         for (int j = 0; j < 2; ++j) mbar_init(&ct->s_full[i][j], 1), mbar_init(&ct->p_full[i][j], 8), mbar_init(&ct->pv_done[i][j], 1);
-        mbar_init(&ct->q_full[i], 8);
+        mbar_init(&ct->q_full[i], kTileConvertWarps);
       }
+      mbar_init(&ct->q_free, 2);
       for (int i = 0; i < P::kRing; ++i) mbar_init(&ct->raw_full[i], 1), mbar_init(&ct->raw_empty[i], kTileConvertWarps / 2);
       fence_mbar_init();
     }
@@ -286,11 +288,52 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     const uint8_t* raw0 = ring + tok * kD + part * 8;
     uint8_t* buf0 = (is_v ? v_buf : k_buf) + dst;
     uint64_t *full = is_v ? ct->v_full : ct->k_full, *empty = is_v ? ct->v_empty : ct->k_empty;
-    uint32_t slot = is_v ? 1 : 0, slot_use = 0, buf = 0, use = 0;
+    uint32_t slot = is_v ? 1 : 0, slot_use = 0, buf = 0, use = 0, units = 0;
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
       at += u.taken;
       if (!u.work) continue;
+      // The unit's q, while the softmax is still at the unit before: the largest value of a row to [2^14, 2^15) by a power of
+      // two, a negative softmax scale into its sign.  A group takes a row tile, or half of the only one; a warp a fourth
+      // of that, kD / 8 lanes a row, so that its loads are whole lines.
+      {
+        constexpr int kLanes = kD / 8, kAtOnce = 32 / kLanes, kRound = 4;
+        const int rows = u.two ? 32 : 16, qt = u.two && is_v ? 1 : 0, row0 = (u.two ? 0 : is_v ? 64 : 0) + cw * rows, c = lane % kLanes;
+        const int my = u.rt * kTileUnitRows + qt * kTileRows + row0 + (lane & (rows - 1)), my_r = my / a.group;  // lane j knows where row j is
+        const int64_t my_at = u.b * a.q_stride_b + my_r * a.q_stride_r + static_cast<int64_t>(u.h * a.group + my - my_r * a.group) * kD;
+        const uint32_t rows_on = __ballot_sync(0xffffffffu, my_r < u.sp.n);
+        uint8_t* dst_q = q_buf + qt * P::kQTile + (c >> 3) * (kTileRows * 128);
+        if (units > 0) tile_wait(&ct->q_free, units - 1, dead);
+#pragma unroll 1
+        for (int i0 = 0; i0 < rows; i0 += kRound * kAtOnce) {
+          uint4 w[kRound];
+#pragma unroll
+          for (int i = 0; i < kRound; ++i) {
+            const int j = i0 + i * kAtOnce + lane / kLanes;
+            const int64_t row_at = __shfl_sync(0xffffffffu, my_at, j);
+            w[i] = make_uint4(0, 0, 0, 0);
+            ld_cg128_if(w[i], a.q + row_at + c * 8, rows_on >> j & 1);
+          }
+#pragma unroll
+          for (int i = 0; i < kRound; ++i) {
+            const int j = row0 + i0 + i * kAtOnce + lane / kLanes;
+            uint32_t m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(0u, w[i].x), w[i].y), w[i].z), w[i].w);
+            m = max(m & 0xFFFFu, m >> 16);
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int e = m ? min(127, 14 - (static_cast<int>(m >> 7) - 127)) : 0;
+            if (c == 0) ct->row_scale[units & 1][qt][j] = pow2i(-e) * fabsf(a.scale_log2);
+            const float up = a.scale_log2 < 0.f ? -pow2i(e) : pow2i(e);
+            *reinterpret_cast<uint4*>(dst_q + j * 128 + (((c & 7) ^ (j & 7)) << 4)) =
+                make_uint4(pack_f16x2(bf16_lo(w[i].x) * up, bf16_hi(w[i].x) * up), pack_f16x2(bf16_lo(w[i].y) * up, bf16_hi(w[i].y) * up),
+                           pack_f16x2(bf16_lo(w[i].z) * up, bf16_hi(w[i].z) * up), pack_f16x2(bf16_lo(w[i].w) * up, bf16_hi(w[i].w) * up));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ct->q_full[units & 1]);
+        ++units;
+      }
       for (int left = 2 * (u.tb - u.ta); left > 0; --left) {
         tile_wait(&ct->raw_full[slot], slot_use, dead);
         uint2 r[P::kPieces];
@@ -411,8 +454,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       at += u.taken;
       if (!u.work) continue;
       const int tiles = u.tb - u.ta, items = u.two ? 2 * tiles : tiles;
-      tile_wait(&ct->q_full[0], units, dead);
-      tile_wait(&ct->q_full[1], units, dead);
+      tile_wait(&ct->q_full[units & 1], units >> 1, dead);
       ++units;
       auto run = [&](auto stream, auto two) {
         constexpr int s = decltype(stream)::value;
@@ -432,6 +474,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
             tc_commit(&ct->s_full[s][odd]);
             tc_commit(&ct->k_empty[buf]);
             if (!both) tc_commit(&ct->k_empty[buf]);  // for the other stream
+            if (i == items - 1) tc_commit(&ct->q_free);
           }
           __syncwarp();
         };
@@ -483,12 +526,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     // The two threads of a row are in warps w and w + 4 of the stream; a barrier of those two (64 threads) is enough.
     const int pair = 2 + s * 4 + (warp & 3);
-    auto tell = [&](int place, float v) {  // place 1: maxima of items; 0: the end's sums, before that the rows' scales
+    auto tell = [&](int place, float v) {  // place 1: maxima of items; 0: the end's sums
       ct->swap[place][s][half][row] = v;
       bar_sync(pair, 64);
       return ct->swap[place][s][half ^ 1][row];
     };
-    uint32_t steps = 0, done = 0;
+    uint32_t steps = 0, done = 0, units = 0;
     for (int64_t at = from; at < end;) {
       const KvTileUnit u = kv_tile_unit(a, prefix, at, end);
       at += u.taken;
@@ -503,50 +546,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         }
         continue;
       }
-      // q: largest value to [2^14, 2^15) by a power of two, a negative softmax scale into its sign.
       // Tokens that the row sees, from this half's first one of the slice on: first .. last - 1; all of the warp's rows see
       // all_first .. all_last - 1.
       const int base = (u.t0 + u.ta) * kTileTokens + half * 32, hi = u.sp.len - u.sp.n + r + 1;
       const int first = on && a.window > 0 ? max(0, hi - a.window) - base : -base, last = (on ? hi : u.sp.len) - base;
       const int all_first = __reduce_max_sync(0xffffffffu, first), all_last = __reduce_min_sync(0xffffffffu, last);
-      // A warp takes 16 of the stream's rows, kD / 8 lanes a row, so that its loads are whole lines (a row to a thread: 9000
-      // cycles); lane j knows where row j is.
-      float qs;
-      {
-        constexpr int kLanes = kD / 8, kAtOnce = 32 / kLanes, kLoads = 16 / kAtOnce;
-        const int row0 = (warp & 7) * 16, c = lane % kLanes, tile_at = u.rt * kTileUnitRows + (u.two ? s : 0) * kTileRows;
-        const int my = tile_at + row0 + (lane & 15), my_r = my / a.group;
-        const int64_t my_at = u.b * a.q_stride_b + my_r * a.q_stride_r + static_cast<int64_t>(u.h * a.group + my - my_r * a.group) * kD;
-        const uint32_t rows_on = __ballot_sync(0xffffffffu, my_r < u.sp.n);
-        uint4 w[kLoads];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int j = i * kAtOnce + lane / kLanes;
-          const int64_t row_at = __shfl_sync(0xffffffffu, my_at, j);
-          w[i] = make_uint4(0, 0, 0, 0);
-          ld_cg128_if(w[i], a.q + row_at + c * 8, rows_on >> j & 1);
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int j = row0 + i * kAtOnce + lane / kLanes;
-          uint32_t m = abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(abs_max_bf16x2(0u, w[i].x), w[i].y), w[i].z), w[i].w);
-          m = max(m & 0xFFFFu, m >> 16);
-#pragma unroll
-          for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const int e = m ? min(127, 14 - (static_cast<int>(m >> 7) - 127)) : 0;
-          if (c == 0) ct->swap[0][s][0][j] = pow2i(-e) * fabsf(a.scale_log2);
-          if (u.two || s == 0) {
-            const float up = a.scale_log2 < 0.f ? -pow2i(e) : pow2i(e);
-            *reinterpret_cast<uint4*>(q_buf + s * P::kQTile + j * 128 + (c >> 3) * (kTileRows * 128) + (((c & 7) ^ (j & 7)) << 4)) =
-                make_uint4(pack_f16x2(bf16_lo(w[i].x) * up, bf16_hi(w[i].x) * up), pack_f16x2(bf16_lo(w[i].y) * up, bf16_hi(w[i].y) * up),
-                           pack_f16x2(bf16_lo(w[i].z) * up, bf16_hi(w[i].z) * up), pack_f16x2(bf16_lo(w[i].w) * up, bf16_hi(w[i].w) * up));
-          }
-        }
-        fence_proxy_async_smem();
-        bar_sync(10 + s, 2 * kTileRows);
-        if (lane == 0) mbar_arrive(&ct->q_full[s]);
-        qs = ct->swap[0][s][0][row];
-      }
+      tile_wait(&ct->q_full[units & 1], units >> 1, dead);
+      const float qs = ct->row_scale[units & 1][u.two ? s : 0][row];
+      ++units;
       const int tiles = u.tb - u.ta, items = u.two ? 2 * tiles : tiles;
       float m = -INFINITY, l = 0.f;
       const uint32_t to = P::o_at(s) + lane_off + half * (kD / 2);
@@ -635,27 +642,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       tc_fence_after();
 
       // A unit that is cut leaves its pieces (O, maximum, sum) to the joining kernel.  One that is not is written here; with
-      // one row tile, stream 1 first hands its sums to stream 0 through the q buffers (every product that reads them is done
-      // once both streams' last are).
+      // one row tile, stream 0 adds stream 1's sums, which it reads from tensor memory.
       const bool cut_unit = u.tb - u.ta != u.tiles, joins = !cut_unit && !u.two;
-      float4* hand = reinterpret_cast<float4*>(q_buf) + half * (kD / 8) * kTileRows;
       float f0 = 1.f, f1 = 0.f;
       if (joins) {
-        if (s == 1) {
-          tile_wait(&ct->pv_done[0][(done - 1) & 1], (done - 1) >> 1, dead);
-          tc_fence_after();
-          if (half == 0) ct->hand[row] = make_float2(m, l);
-#pragma unroll
-          for (int c = 0; c < kD / 64; ++c) {
-            uint32_t x[32];
-            tmem_ld32(x, to + c * 32);
-            tmem_wait_ld(x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) hand[(c * 8 + i) * kTileRows + row] = make_float4(
-                __uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3]));
-          }
-        }
+        if (s == 1 && half == 0) ct->hand[row] = make_float2(m, l);
+        tc_fence_before();
         bar_sync(1, kTileSoftmax);
+        tc_fence_after();
         if (s == 0) {
           const float2 o = ct->hand[row];
           const float mn = fmaxf(m, o.x);
@@ -667,27 +661,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       if (!(joins && s == 1)) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t slot = kv_tile_slot(blockIdx.x, u.ta == 0, s);
-#pragma unroll
-        for (int c = 0; c < kD / 64; ++c) {
-          uint32_t x[32];
-          tmem_ld32(x, to + c * 32);
+#pragma unroll 1
+        for (int c = 0; c < kD / 32; ++c) {
+          uint32_t x[16];
+          tmem_ld16(x, to + c * 16);
           tmem_wait_ld(x);
           if (cut_unit) {
             if (on) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                __stcg(a.part + (slot * (kD / 4) + half * (kD / 8) + c * 8 + i) * kTileRows + row,
+              for (int i = 0; i < 4; ++i)
+                __stcg(a.part + (slot * (kD / 4) + half * (kD / 8) + c * 4 + i) * kTileRows + row,
                        make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])));
             }
-          } else if (exists) {
-            uint2* o = reinterpret_cast<uint2*>(a.o + out_row * kD + half * (kD / 2) + c * 32);
+          } else {
+            if (joins) {
+              uint32_t y[16];
+              tmem_ld16(y, P::o_at(1) + lane_off + half * (kD / 2) + c * 16);
+              tmem_wait_ld(y);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (joins) v = hand[(c * 8 + i) * kTileRows + row];
-              const float y0 = fmaf(__uint_as_float(x[4 * i]), f0, v.x * f1), y1 = fmaf(__uint_as_float(x[4 * i + 1]), f0, v.y * f1);
-              const float y2 = fmaf(__uint_as_float(x[4 * i + 2]), f0, v.z * f1), y3 = fmaf(__uint_as_float(x[4 * i + 3]), f0, v.w * f1);
-              o[i] = on ? make_uint2(pack_bf16x2(y0 * inv, y1 * inv), pack_bf16x2(y2 * inv, y3 * inv)) : make_uint2(0u, 0u);
+              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f0 + __uint_as_float(y[i]) * f1);
+            }
+            if (exists) {
+              uint2* o = reinterpret_cast<uint2*>(a.o + out_row * kD + half * (kD / 2) + c * 16);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                o[i] = on ? make_uint2(pack_bf16x2(__uint_as_float(x[4 * i]) * inv, __uint_as_float(x[4 * i + 1]) * inv),
+                                       pack_bf16x2(__uint_as_float(x[4 * i + 2]) * inv, __uint_as_float(x[4 * i + 3]) * inv))
+                          : make_uint2(0u, 0u);
             }
           }
         }
@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         }
       }
       tc_fence_before();
-      bar_sync(1, kTileSoftmax);  // the q buffers are written again by the next unit
+      if (joins) bar_sync(1, kTileSoftmax);  // (stream 1's sums have been read)
     }
   }
   __syncthreads();

@@ -74,22 +74,24 @@ cudaError_t run_rope(const RopeArgs& a, bool interleaved, cudaStream_t s) {
 
 // How a call's rows (query tokens x heads of one kv head) are taken: 8 or 16 at a time by the streaming kernel, or 256 at a
 // time by the tile kernel, when there are many rows and much work: the streaming kernel reads a cache once per 16 rows, the
-// tile kernel costs 20 to 30 us in any case (two launches, a pipeline to fill).  Work is what the streaming kernel's line
-// would hold at most, from the page table's width and the window: lengths are on the device.
-// 16 sequences of 801 to 9001 tokens, 8 kv heads, streaming / tile in us, by rows:
-//   128 values: 16 rows 58 / 85, 24 rows 99 / 87, 48 rows 142 / 91; one sequence of 65001: 32 rows 80 / 95, 48 rows 108 / 96
-//   64 values: 32 rows 61 / 82, 48 rows 85 / 83, 64 rows 110 / 83; one sequence of 65001: 48 rows 60 / 80, 96 rows 105 / 82
-// and of the work, in tiles of the line per SM:
-//   128 values, one sequence: 512 rows, 801 tokens (142) 30 / 38; 128 rows, 6401 tokens (187) 40 / 44; 512 rows, 1601 tokens (230) 43 / 39
-//   64 values, one sequence: 512 rows, 1601 tokens (230) 27 / 31; 2048 rows, 256 tokens (330) 31 / 29; 512 rows, 3201 tokens (400) 38 / 33
+// tile kernel costs 20 us in any case (two launches, a pipeline to fill).  Work is what the streaming kernel's line would
+// hold at most, from the page table's width and the window: lengths are on the device.
+// Streaming / tile in us, 8 kv heads, 16 sequences of 801 to 9001 tokens, and one of 65001:
+//   128 values: 16 rows 58 / 83, 55 / 72; 24 rows 99 / 84, 80 / 73; 48 rows 142 / 87, 108 / 74
+//   64 values: 16 rows 36 / 73, 33 / 60; 32 rows 61 / 73, 46 / 61; 48 rows 85 / 74, 60 / 61; 96 rows 159 / 76, 105 / 62
+// and by work, in tiles of the line per SM:
+//   128 values: 128 rows, 3201 tokens (100) 28 / 27; 512 rows, 801 tokens (143) 30 / 36; 128 rows, 6401 tokens (187) 40 / 30;
+//   512 rows, 1601 tokens (230) 43 / 37
+//   64 values: 128 rows, 6401 tokens (187) 24 / 25; 512 rows, 1601 tokens (230) 27 / 31; 16 sequences, 128 rows, 201 tokens (311)
+//   31 / 17; 512 rows, 3201 tokens (400) 38 / 32
 // 8 rows of 128 values taken as 16: 57 -> 84 us (one sequence of 131071 tokens).
 struct AttentionPlan {
   bool tile;
   int rows;            // of a unit
   int64_t row_tiles;   // units per kv head
 };
-int64_t tile_work(int64_t D, int sms) { return sms * (D == 64 ? 300ll : 200ll); }
-bool tile_rows(int64_t B, int64_t rows, int64_t D) { return ((D == 64 && rows > 48) || (D == 128 && rows > 32)) && B <= kTileMaxBatch; }
+int64_t tile_work(int64_t D, int sms) { return sms * (D == 64 ? 250ll : 150ll); }
+bool tile_rows(int64_t B, int64_t rows, int64_t D) { return ((D == 64 && rows > 32) || (D == 128 && rows > 16)) && B <= kTileMaxBatch; }
 AttentionPlan stream_plan(int64_t rows) {
   const int unit = rows <= 8 ? 8 : 16;
   return {false, unit, (rows + unit - 1) / unit};
