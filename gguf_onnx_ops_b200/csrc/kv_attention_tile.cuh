@@ -596,14 +596,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
           if (i > 0) {
             tile_wait(&ct->pv_done[s][(g - 1) & 1], (g - 1) >> 1, dead);
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < kD / 32; ++c) {
-              uint32_t y[16];
-              tmem_ld16(y, to + c * 16);
+#pragma unroll 1
+            for (int c = 0; c < kD / 2; c += 8) {  // (rare: few registers and little code, or the loop around it pays)
+              uint32_t y[8];
+              tmem_ld8(y, to + c);
               tmem_wait_ld(y);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
-              tmem_st16(to + c * 16, y);
+              for (int j = 0; j < 8; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
+              tmem_st8(to + c, y);
             }
           }
         }
