@@ -537,9 +537,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       at += u.taken;
       const int rr = u.rt * kTileUnitRows + (u.two ? s : 0) * kTileRows + row, r = rr / a.group;
       const bool on = r < u.sp.n, exists = r < a.R;
-      const int64_t out_row = (static_cast<int64_t>(u.b) * a.R + r) * a.heads + u.h * a.group + rr % a.group;
+      auto out_row_of = [&] {
+        const int rr = u.rt * kTileUnitRows + (u.two ? s : 0) * kTileRows + row, r = rr / a.group;
+        return (static_cast<int64_t>(u.b) * a.R + r) * a.heads + u.h * a.group + (rr - r * a.group);
+      };
       if (!u.work) {  // none of the unit's rows sees anything (or the slice ends before its tiles)
         if (u.mine && exists && (u.two || s == 0)) {
+          const int64_t out_row = out_row_of();
           uint4* o = reinterpret_cast<uint4*>(a.o + out_row * kD) + half * (kD / 16);
           for (int i = 0; i < kD / 16; ++i) o[i] = make_uint4(0, 0, 0, 0);
           if (a.lse && half == 0) a.lse[out_row] = -INFINITY;
@@ -606,6 +610,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
               tmem_st8(to + c, y);
             }
           }
+          tmem_ld32(x, ts + half * 32);  // (read again rather than kept over all this; weights go over them after both have)
+          tmem_wait_ld(x);
+          bar_sync(pair, 64);
         }
         const float top = m == -INFINITY ? 0.f : m - kTileTop;
         uint32_t w[16];
@@ -659,6 +666,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         }
       }
       if (!(joins && s == 1)) {
+        const int64_t out_row = out_row_of();
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t slot = kv_tile_slot(blockIdx.x, u.ta == 0, s);
 #pragma unroll 1
