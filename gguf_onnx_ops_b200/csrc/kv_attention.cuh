@@ -14,10 +14,14 @@
 // of it, which is what the factor 2^15 is for.
 //
 // Work.  The cache positions of all (sequence, kv head, row tile) units are laid out in one line of 16-token tiles, with a
-// stretch for each unit's own cost before them, and cut into equal slices, one per CTA, whatever the lengths are; lengths are read on the device, so a captured graph serves
-// any of them.  The eight warps of a CTA take its tiles in turn, each with its own statistics, and meet at the end of
+// stretch for each unit's own cost before them, and cut into equal slices, one per CTA, whatever the lengths are; lengths
+// are read on the device, so a captured graph serves any of them.  The eight warps of a CTA take its tiles in turn, each with its own statistics, and meet at the end of
 // the unit; a unit cut between CTAs leaves its pieces in the workspace, and the CTA that finishes last (a counter per
 // unit) joins them in order, so results do not depend on timing.
+//
+// Bound.  Memory for many sequences (64 of 131 to 8009 tokens, 8 kv heads of 128: 99 us, 5.4 TB/s); for one of 131071
+// tokens the conversion of the codes shares it (57 us, 4.7 TB/s; the ALU pipe 52 % busy); few tokens are a chain of loads
+// (lens, table, page, rows, pieces: 10 us for 777 tokens).  16 rows take half as long again as 8 (85 us against 57).
 //
 // A tile's fragments: S^T (16 tokens x 8 rows) = K (A operand) q^T (B), so that K goes straight from global memory
 // into the A fragment: lane (g, t) loads 16 consecutive bytes of rows g and g + 8, and the order of the head's values

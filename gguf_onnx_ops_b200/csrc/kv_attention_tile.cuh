@@ -1,22 +1,31 @@
 // Attention of many query rows over the 8-bit paged KV cache: 128-row tiles on tcgen05 (the formulas, the scaling of q
 // and the use of V's page scale are those of kv_attention.cuh; w_j <= 2^15 here too, kept so by a running maximum that moves
-// only when it has grown by more than 2^4, with weights scaled to 2^11).
+// only when it has grown by more than 2^4, with weights scaled to 2^11: f16 rounds a weight by 2^-12 of it, or by 2^-36 of the
+// largest for weights below 2^-25 of it).
 //
 // Why.  R * heads / kv_heads rows share the K and V of a kv head.  The streaming kernel converts the codes once per 16
-// rows and multiplies on mma.sync; from 17 rows on that work, not the bytes, is its time (48 rows, 16 sequences of up to 9001
-// tokens: 265 us for 25 us of bytes).  Here a CTA converts each 128-token tile of codes once, to f16 in shared
+// rows and multiplies on mma.sync; from 17 rows on that work, not the bytes, is its time (48 rows, 16 sequences of 801 to 9001
+// tokens: 142 us for 25 us of bytes, 79 us here).  Here a CTA converts each 128-token tile of codes once, to f16 in shared
 // memory, for up to 256 rows, and the products run on the 5th-generation tensor cores.
 //
 // One CTA per SM, seven warp groups; the tokens go by in steps of 64:
 //   warps 0-7, 8-15  softmax of stream 0 and 1: two threads per row, scores and O in tensor memory
-//   warps 16-19, 20-23  K and V codes to f16, stored swizzled for the MMAs: three buffers each; warp 27 the page scales
+//   warps 16-19, 20-23  K and V codes to f16, stored swizzled for the MMAs: three buffers each; and a unit's q
+//   warp 27          page scales
 //   warp 25          copies codes into a ring of steps (bulk copies, a page each: loads through the L1 stop at what the
 //                    28 KB beside this much shared memory hold, 2 us a tile)
-//   warps 24 and 26  issue the MMAs of a stream: S = q K^T (128 x 64), then O += w V with w (f16) in the columns of its S.  Every stream
-//                    has two S, so that the next scores are there before this step's weights are done
+//   warps 24 and 26  issue the MMAs of a stream: S = q K^T (128 x 64), then O += w V with w (f16) in the columns of its S.
+//                    Every stream has two S, so that the next scores are there before this step's weights are done (one S
+//                    and two places for weights: a step of a chunk 5 % longer)
 // A stream is a 128-row tile against every step when a unit has two row tiles (256 rows share the converted codes), or
 // one row tile against every second step when it has one (two accumulators, joined at the end).
 // The line of all units' 128-token tiles is cut into equal slices as in the streaming kernel; a second kernel joins the pieces.
+//
+// Bound.  A step of two streams takes about 2300 cycles: the softmax warps' instructions (issue slots 58 % used, the exp unit
+// 38 %) and the round of waits between them and the MMAs (tensor pipe 36 %).  A chunk of 1001 tokens, 32 heads over 8 kv
+// heads of 128, 9001 positions: 187 us, 745 TFLOP/s, 16 us of it the joining kernel.  A unit's begin and end take 5000
+// cycles each, a launch 15000 before the first step, which is what few tokens cost.  With parts left out (of 195 us before
+// the last steps): 172 us without exponentials, 180 with an eighth of S's products, no less without the conversion of the codes.
 #pragma once
 
 #include <type_traits>

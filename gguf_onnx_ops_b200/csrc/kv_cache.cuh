@@ -71,13 +71,6 @@ __device__ __forceinline__ bool kv_page_ok(const KvPages& c, int entry) {
   record_device_error(kSiteBadCachePage);
   return false;
 }
-// Page of stretch i of sequence b, or -1 (recorded) where the table or the page is out of range.
-__device__ __forceinline__ int64_t kv_page(const KvPages& c, int b, int i) {
-  int p = -1;
-  if (i < c.table_cols) p = ld_cg(c.table + static_cast<int64_t>(b) * c.table_cols + i);
-  return kv_page_ok(c, p) ? p : -1;
-}
-
 struct KvWriteArgs {
   KvPages c;
   const bf16* x[2];  // K and V: [B, R, kv_heads, D], strides in values
@@ -110,7 +103,7 @@ __device__ __forceinline__ uint32_t abs_max_bf16x2(uint32_t m, uint32_t w) { ret
 
 // One CTA per (touched page, head, K or V) of a sequence: blockIdx = (page of the call * 2 + which, head, sequence).  The
 // call's tokens of the page stay in registers between the maximum and the codes (16 KB at 64 tokens of 128 values); loads
-// that do not depend on one another are issued before any is used.
+// that do not depend on one another are issued before any is used: what is left in turn is lens, table entry, page.
 template <int kD>
 __global__ void __launch_bounds__(kKvWriteThreads) kv_write_kernel(const KvWriteArgs a) {
   constexpr int kPer = kD / 8;  // 16-byte pieces of a token

@@ -214,10 +214,11 @@ int gguf_qk_norm_rope(const void* x, const float* gamma_q, const float* gamma_k,
                    static_cast<bf16*>(k), row_stride, T, static_cast<int>(heads), static_cast<int>(kv_heads),
                    static_cast<int>(head_dim), static_cast<int>(rot), static_cast<int>(max_pos), eps};
   auto* s = static_cast<cudaStream_t>(stream);
-  // One head per lane group while the call does not fill the GPU, four after that (their loads overlap, and cos, sin
-  // and gamma are read once for the four: 8191 tokens 32.9 us against 43).
+  // One head per lane group while the call does not fill the GPU, four after that (their loads overlap, and cos, sin and
+  // gamma are read once for the four).  40 heads of 128, one / four, in us: 1 token 1.8 / 2.4, 128 tokens 2.4 / 2.6, 256 tokens
+  // 3.2 / 2.9, 8191 tokens 43 / 33.
   const int lanes = head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32;
-  const bool few = T * (heads + kv_heads) * lanes <= static_cast<int64_t>(sms) * 2048;
+  const bool few = T * (heads + kv_heads) * lanes <= static_cast<int64_t>(sms) * 1024;
   const bool in = interleaved != 0;
   cudaError_t e;
   if (lanes == 8) e = few ? run_rope<8, 1>(a, in, s) : run_rope<8, 4>(a, in, s);
@@ -351,7 +352,8 @@ int gguf_draft_verify(const float* target, const float* draft_probs, const int32
   const bool wide = V % 4 == 0 && is_aligned(target, 16) && (!draft_probs || is_aligned(draft_probs, 16));
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  // A sequence's row is shared by as many CTAs (8 at most) as keep the whole call in one wave of two an SM.
+  // A sequence's row is shared by as many CTAs (8 at most) as keep the whole call in one wave of two an SM.  131072 tokens, 8
+  // / 4 / 1 CTAs, in us: 16 sequences 8.5 / - / 26; 64 sequences 18.5 / 13.9 / 31.  32000 tokens, 256 sequences: 8 CTAs 47, one 13.5.
   int ctas = kDraftCtas;
   while (ctas > 1 && B * ctas > 2 * sms) ctas /= 2;
   cudaLaunchConfig_t cfg = {};

@@ -7,7 +7,7 @@
 // A group of kGL lanes owns one head: lane l holds eight of its values as two 8-byte pieces, chosen so that both members of
 // a pair sit in the same lane (no shuffles beyond the sum of squares), and the same two pieces of every head of a token use
 // the same four cos and sin values, which are loaded once for the kHeads heads that a group works on.  Bound by memory: 8191
-// tokens of 32 + 8 heads of 128 take 32.9 us (5.2 TB/s); one head a group 43 us, 16-byte pieces on half the lanes 34.6 us.
+// tokens of 32 + 8 heads of 128 take 33 to 34 us (5.2 TB/s); one head a group 43 us, 16-byte pieces on half the lanes 34.6 us.
 #pragma once
 
 #include "kv_cache.cuh"
