@@ -73,19 +73,22 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
     rope_floats(ga, gamma + oa);
     rope_floats(gb, gamma + ob);
   }
+  // A warp holds groups of queries and of keys: where only one of the two has a norm, all its lanes still take part in the
+  // sums (the others' factor is 1), since the shuffles name the whole warp.
+  const bool norms = a.gq || a.gk;
   const float rd = 1.0f / static_cast<float>(a.D);
   bf16* out = (is_q ? a.q : a.k) + (static_cast<int64_t>(t) * hn + h0) * a.D;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     float x[4] = {bf16_lo(va[i].x), bf16_hi(va[i].x), bf16_lo(va[i].y), bf16_hi(va[i].y)};
     float z[4] = {bf16_lo(vb[i].x), bf16_hi(vb[i].x), bf16_lo(vb[i].y), bf16_hi(vb[i].y)};
-    if (gamma) {
+    if (norms) {
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) ss += x[j] * x[j] + z[j] * z[j];
 #pragma unroll
       for (int o = kGL / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(ss * rd + a.eps);
+      const float r = gamma ? rsqrtf(ss * rd + a.eps) : 1.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] *= r * ga[j], z[j] *= r * gb[j];
     }

@@ -80,6 +80,26 @@ def test_without_norm_strided_rows_and_leading_dims(cuda):
     assert e[0].shape == (0, hq, D)
 
 
+@pytest.mark.parametrize("T", [3, 700])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q_norm,k_norm", [(False, True), (True, False), (False, False)])
+def test_a_norm_on_one_side_only(cuda, T, D, q_norm, k_norm):
+    """A warp has query and key heads side by side, with one head a lane group (few tokens) and with four; heads without a
+    norm come out as their rounded rotation, whatever the others have."""
+    g = gen(T + D)
+    hq, hk = 5, 3
+    qkv = (torch.randn(T, (hq + 2 * hk) * D, generator=g) * 2).to(torch.bfloat16).to(cuda)
+    gq = (torch.rand(D, generator=g) + 0.5).to(cuda) if q_norm else None
+    gk = (torch.rand(D, generator=g) + 0.5).to(cuda) if k_norm else None
+    cos, sin = tables(301, D, cuda)
+    pos = torch.randint(0, 301, (T,), generator=g, dtype=torch.int32).to(cuda)
+    got = ops.QkNormRope(qkv, gq, gk, cos, sin, pos, heads=hq, kv_heads=hk)
+    check(got, *reference(qkv, gq, gk, cos, sin, pos, hq, hk, 1e-6, False))
+    bare = ops.QkNormRope(qkv, None, None, cos, sin, pos, heads=hq, kv_heads=hk)
+    for y, z, norm in zip(got, bare, (q_norm, k_norm)):
+        assert norm or torch.equal(y, z)
+
+
 def test_extreme_rows(cuda):
     """Zero heads, tiny and huge values; an infinite value makes its own head NaN and no other."""
     hq, hk, D = 3, 1, 64
