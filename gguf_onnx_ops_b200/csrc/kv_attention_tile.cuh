@@ -472,8 +472,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
           const uint32_t odd = __shfl_sync(0xffffffffu, (done + i) & 1, 0);
           buf = __shfl_sync(0xffffffffu, buf, 0);
           tile_wait(&ct->k_full[buf], use, dead);
-          if (i > 1) tile_wait(&ct->pv_done[s][odd], (done + i - 2) >> 1, dead);  // the weights over this S are used (all of
-          tc_fence_after();                                                       // them, at a unit's begin)
+          // The weights over this S are used: those of the item two before, of the last unit's too (its products with V were
+          // issued after the last scores, which are all that q_full stands for).
+          if (done + i > 1) tile_wait(&ct->pv_done[s][odd], (done + i - 2) >> 1, dead);
+          tc_fence_after();
           if (elect_one()) {
             const uint64_t kd = k_desc + buf * (P::kOperand >> 4);
 #pragma unroll

@@ -88,6 +88,15 @@ def test_many_rows(cuda, R):
     run_case(cuda, 3, R, 4, 2, 256, 64, [R, R + 3, 900], seed=R, news=[R, 3, R // 2])
 
 
+@pytest.mark.parametrize("R,D", [(40, 128), (70, 64), (300, 128)])
+def test_units_follow_one_another_in_a_block(cuda, R, D):
+    """More (sequence, kv head) units than blocks, of one to a few 64-token steps each: a unit's first scores go where the
+    last unit's weights were.  The lengths leave odd and even numbers of steps; one and two row tiles."""
+    B = 60 if R < 100 else 24
+    lens = [R + (61 * i) % 530 for i in range(B)]
+    run_case(cuda, B, R, 8, 8, 64, D, lens, news=[R if i % 5 else 1 + i % R for i in range(B)], seed=R)
+
+
 def test_one_long_sequence(cuda):
     run_case(cuda, 1, 1, 8, 2, 64, 128, [40007], seed=1)
     run_case(cuda, 1, 2, 4, 1, 64, 64, [70001], seed=2, window=60000)
