@@ -647,14 +647,16 @@ def KvCacheRead(cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor, *,
 
 class KvAttentionWorkspace:
     """Scratch of KvCacheAttention calls that do not overlap: partial results, and counters that are zero between calls.
-    Grows to the largest call it has served."""
+    Grows to the largest call it has served.  What it has outgrown is kept as long as the workspace: a captured graph goes on
+    using what it was captured with (so keep the workspace as long as the graph), and a call on another stream may not be
+    done with it."""
 
-    __slots__ = ("device", "scratch", "counters", "_sizes", "_captured")
+    __slots__ = ("device", "scratch", "counters", "_sizes", "_captured", "_outgrown")
 
     def __init__(self, device, _captured: bool = False):
         self.device, self._captured = device, _captured
         self.scratch = self.counters = None
-        self._sizes = {}
+        self._sizes, self._outgrown = {}, []
 
     def fit(self, B: int, R: int, heads: int, kv_heads: int, head_dim: int) -> "KvAttentionWorkspace":
         key = (B, R, heads, kv_heads, head_dim)
@@ -663,10 +665,14 @@ class KvAttentionWorkspace:
                 raise ValueError("KvCacheAttention: call fit() of a workspace before it is used in a capture")
             nbytes, n = ctypes.c_int64(0), ctypes.c_int64(0)
             check(load().gguf_kv_cache_attention_workspace(*key, ctypes.byref(nbytes), ctypes.byref(n)))
+            # (a handful of scratch sizes exist, and counters at least double: what is kept stays small)
             if self.scratch is None or self.scratch.numel() < nbytes.value:
+                self._outgrown.append(self.scratch)
                 self.scratch = torch.empty(nbytes.value, dtype=torch.uint8, device=self.device)
             if self.counters is None or self.counters.numel() < n.value:
-                self.counters = torch.zeros(max(n.value, 1024), dtype=torch.int32, device=self.device)
+                self._outgrown.append(self.counters)
+                most = 1024 if self.counters is None else 2 * self.counters.numel()
+                self.counters = torch.zeros(max(n.value, most), dtype=torch.int32, device=self.device)
             self._sizes[key] = True
         return self
 

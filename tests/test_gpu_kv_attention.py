@@ -223,6 +223,34 @@ def test_captured_graph_serves_other_lengths(cuda, R, extra):
             check(out, ref, mag, c, case)
 
 
+def test_a_workspace_that_grows_leaves_captured_graphs_what_they_use(cuda):
+    B, R, H, Hk, page, D = 2, 2, 8, 2, 64, 128
+    c = K.make_cache(120, Hk, page, D, 14, cuda)
+    cache, case = ops.KvCache(*c), [3000, 2900]
+    table = K.make_table(B, 50, 120, 15, cuda)
+    q = torch.randn(B, R, H, D, generator=K.gen(16)).to(torch.bfloat16).to(cuda)
+    lens = torch.tensor(case, dtype=torch.int32, device=cuda)
+    ws = ops.KvAttentionWorkspace(cuda).fit(B, R, H, Hk, D)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.KvCacheAttention(q, cache, table, lens, workspace=ws)
+    small = [(t.data_ptr(), t.numel() * t.element_size()) for t in (ws.scratch, ws.counters)]
+    ws.fit(64, 300, 32, 8, D)
+    assert ws.scratch.numel() > small[0][1] and ws.counters.numel() * 4 > small[1][1]
+    # Allocations of the same sizes get other memory, and the replays leave them alone.
+    others = [torch.full((n,), 77, dtype=torch.uint8, device=cuda) for _, n in small for _ in range(8)]
+    for t in others:
+        for at, n in small:
+            assert t.data_ptr() + t.numel() <= at or at + n <= t.data_ptr()
+    ref, mag, _ = K.attention(q, c, table, case, None, D ** -0.5, 0)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        check(out, ref, mag, c, case)
+        check(ops.KvCacheAttention(q, cache, table, lens, workspace=ws), ref, mag, c, case)
+    assert all((t == 77).all() for t in others)
+
+
 def test_lengths_past_the_table_are_reported(cuda):
     c = K.make_cache(4, 1, 16, 64, 1, cuda)
     q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device=cuda)
