@@ -364,8 +364,9 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
         }
         const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] - kKvTop, m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] - kKvTop;
         const float w0 = ex2(x[0] - m0), w1 = ex2(x[1] - m1), w2 = ex2(x[2] - m0), w3 = ex2(x[3] - m1);
-        l[nt][0] = fmaf(w0 + w2, inv_v, l[nt][0]);
-        l[nt][1] = fmaf(w1 + w3, inv_v, l[nt][1]);
+        // (a row that sees none of the tile adds nothing: the page's scale may be anything there, and its weights are 0)
+        if (w0 + w2 != 0.f) l[nt][0] = fmaf(w0 + w2, inv_v, l[nt][0]);
+        if (w1 + w3 != 0.f) l[nt][1] = fmaf(w1 + w3, inv_v, l[nt][1]);
         pb[nt][0] = movmatrix_trans(pack_f16x2(w0, w1));
         pb[nt][1] = movmatrix_trans(pack_f16x2(w2, w3));
       }
