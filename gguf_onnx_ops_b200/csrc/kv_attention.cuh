@@ -225,30 +225,31 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
     const int lg = a.c.log2_page, in_page = (1 << lg) - 1;
     const int32_t* table = a.c.table + static_cast<int64_t>(b) * a.c.table_cols;  // (positions below len lie in it)
     uint32_t entry = 0, entry_next = 0;  // pages of `tile` and of this warp's next tile
-    auto page_of = [&](uint32_t e) { return static_cast<int64_t>(kv_page_ok(a.c, static_cast<int>(e)) ? e : 0); };
-    auto row0 = [&](int64_t page, int tl) {
-      return ((((page * a.c.kv_heads + h) << lg) + ((tl * kKvTile) & in_page))) * kD;
+    // -1: not in the cache; nothing is loaded then, and the tile is hidden from every row
+    auto page_of = [&](uint32_t e) { return kv_page_ok(a.c, static_cast<int>(e)) ? static_cast<int>(e) : -1; };
+    auto row0 = [&](int page, int tl) {
+      return (((static_cast<int64_t>(page) * a.c.kv_heads + h) << lg) + ((tl * kKvTile) & in_page)) * kD;
     };
-    auto load_k = [&](int64_t page, int tl, bool on) {
+    auto load_k = [&](int page, int tl, bool on) {
       const int8_t* p = a.k + row0(page, tl) + t * P::kKPiece;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int j = 0; j < kD / (4 * P::kKPiece); ++j)
           load_codes_if<P::kKPiece>(&kw[r][j * (P::kKPiece / 4)], p + (g + 8 * r) * kD + j * 4 * P::kKPiece, on);
-      ld_cg32_if(ks, a.ks + page * a.c.kv_heads + h, on);
-      ld_cg32_if(vs, a.vs + page * a.c.kv_heads + h, on);
+      ld_cg32_if(ks, a.ks + static_cast<int64_t>(page) * a.c.kv_heads + h, on);
+      ld_cg32_if(vs, a.vs + static_cast<int64_t>(page) * a.c.kv_heads + h, on);
     };
-    auto load_v = [&](int64_t page, int tl, bool on) {
+    auto load_v = [&](int page, int tl, bool on) {
       const int8_t* p = a.v + row0(page, tl) + g * (kD / 8);
 #pragma unroll
       for (int r = 0; r < 4; ++r) load_codes_if<kD / 8>(vw[r], p + (2 * t + (r & 1) + 8 * (r >> 1)) * kD, on);
     };
     ld_cg32_if(entry, table + ((tile * kKvTile) >> lg), tile < stop);
     ld_cg32_if(entry_next, table + (((tile + kKvWarps) * kKvTile) >> lg), tile + kKvWarps < stop);
-    int64_t page = page_of(entry);
-    load_k(page, tile, tile < stop);
-    load_v(page, tile, tile < stop);
+    int page = page_of(entry);
+    load_k(page, tile, tile < stop && page >= 0);
+    load_v(page, tile, tile < stop && page >= 0);
 
     // Rows: q as f16 fragments, their limits.
     for (int n = warp; n < P::kRows; n += kKvWarps) {
@@ -321,15 +322,16 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
         }
       }
       const float ks_now = __uint_as_float(ks), vs_now = vs << 1 == 0 ? 1.f : __uint_as_float(vs);
-      const bool more = next < stop;
+      const bool more = next < stop, here = page >= 0;
       page = page_of(entry_next);  // (read a tile ahead; page 0 where there is no next tile)
-      load_k(page, next, more);
+      const bool loads = more && page >= 0;
+      load_k(page, next, loads);
       entry_next = more ? entry_next : 0;
       ld_cg32_if(entry_next, table + (((next + kKvWarps) * kKvTile) >> lg), next + kKvWarps < stop);
 
       const float lv = lg2(vs_now), inv_v = __fdividef(1.0f, vs_now);
       const int p0 = tile * kKvTile;
-      const bool whole = p0 >= all_lo && p0 + kKvTile <= all_hi;
+      const bool whole = p0 >= all_lo && p0 + kKvTile <= all_hi && here;
       uint32_t pb[kNT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int pos = p0 + g + 8 * (i >> 1);
-            if (pos < lo[nt][i & 1] || pos >= hi[nt][i & 1]) x[i] = -INFINITY;
+            if (pos < lo[nt][i & 1] || pos >= hi[nt][i & 1] || !here) x[i] = -INFINITY;
           }
         }
         float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
           for (int nt = 0; nt < kNT; ++nt) mma_f16_16816(o[nt][2 * j + k], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
         }
       }
-      load_v(page, next, more);
+      load_v(page, next, loads);
       tile = next;
     }
 

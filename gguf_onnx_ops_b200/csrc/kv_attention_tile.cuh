@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
     } else if (warp == kTileMmaWarp + 3) {
     // ---------------------------------------------------------------- page scales
     // Of a step's four groups of 16 tokens (pages hold whole groups), read two steps ahead: lanes 0-3 K's, lanes 4-7 V's.
-    // A page outside the cache (the copying warp records it) counts as zeros.  K's buffer counts as filled when they are
+    // A page outside the cache (the copying warp records it) gets the scales 0 and log2 of 0: the logits of its tokens are
+    // -inf whatever older codes the buffers hold for them.  K's buffer counts as filled when the scales are
     // there too: the softmax reads them once S is.  (Their slot was last read for the step eight before; the products with
     // K's buffer that are waited for here were issued after that step's weights had been used.)
     const int lg = a.c.log2_page;
@@ -432,7 +433,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         return w;
       };
       int st = 2 * (u.t0 + u.ta);
-      uint32_t scale = scale_of(entry_of(st)), entry_next = entry_of(st + 1);
+      const uint32_t entry = entry_of(st);
+      uint32_t scale = scale_of(entry), entry_next = entry_of(st + 1);
+      bool here = entry < a.c.pages;
       for (; st < st_end; ++st, ++steps) {
         const uint32_t buf = steps % kTileBufs, use = steps / kTileBufs;
         if (use > 0) tile_wait(&ct->k_empty[buf], use - 1, dead);
@@ -440,10 +443,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
           ct->scale_k[steps & 7][lane] = __uint_as_float(scale);
         } else if (lane < 8) {
           const float sv = scale << 1 == 0 ? 1.f : __uint_as_float(scale);
-          ct->lv[steps & 7][lane & 3] = lg2(sv);
+          ct->lv[steps & 7][lane & 3] = here ? lg2(sv) : -INFINITY;
           ct->inv_v[steps & 7][lane & 3] = __fdividef(1.f, sv);
         }
         scale = scale_of(entry_next);
+        here = entry_next < a.c.pages;
         entry_next = entry_of(st + 2);
         __syncwarp();
         if (lane == 0) mbar_arrive(&ct->k_full[buf]);

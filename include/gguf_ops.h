@@ -304,7 +304,8 @@ GGUF_OPS_API int gguf_qk_norm_rope(const void* x, const float* gamma_q, const fl
  * stretch of `page` tokens; lens i32 [B] is each sequence's length, a call's new tokens included (they are its last
  * n: n = new_lens[b], or R where new_lens is NULL, never more than lens[b]).
  * Contract: head_dim 64, 96, 128, 192 or 256; page 16, 32, 64, 128 or 256; codes 16-byte aligned.  A page number or a
- * length outside the cache is skipped and reported through gguf_device_status.
+ * length outside the cache is skipped (its positions are not written, are read as 0 and are hidden from attention) and
+ * reported through gguf_device_status.
  */
 typedef struct {
   void *k, *v;               /* int8 [pages, kv_heads, page, head_dim] */

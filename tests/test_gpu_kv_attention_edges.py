@@ -120,3 +120,25 @@ def test_a_marked_page_that_the_window_hides(cuda, form):
     assert sees[:, 0].all() and (R < 20 or not sees[:, 16:].any())
     check(out, lse, ref, cache, table, lens)
     assert torch.isnan(out[sees]).all()
+
+
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+@pytest.mark.parametrize("page", [16, 64])
+def test_pages_outside_the_cache_are_skipped(cuda, form, page):
+    """Positions of such a page do not count, whatever page 0 or an earlier step holds; a sequence of nothing else gives 0."""
+    R = form[1]
+    lens = [R + 7 * page + 5, R + 3 * page, R + 2]
+
+    def edit(c, table):
+        n = c[0].shape[0]
+        table[0, 1], table[0, 4], table[1, 0] = -1, n, 1 << 30
+        table[2] = -7
+        for x in c[2:]:
+            x[0] = 1e4  # page 0 shows where it is taken in
+
+    ops.device_status()
+    out, lse, ref, cache, table = call(cuda, form, lens, page=page, edit=edit, seed=3)
+    assert ops.device_status() == (4, 7)
+    assert torch.isfinite(ref[0]).all() and (ref[0][2] == 0).all()
+    check(out, lse, ref, cache, table, lens)
+    assert (out[2] == 0).all()
