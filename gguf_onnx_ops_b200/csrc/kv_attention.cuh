@@ -9,7 +9,8 @@
 // running maximum, the sum and the output accumulators are fp32.  With s_j the base-2 logit and a_j the V scale of
 // token j's page, the kernel keeps m = max_j (s_j + log2 a_j) and w_j = 2^(s_j + log2 a_j - m + 15) <= 2^15: the page
 // scale of V is part of the exponent, so w_j in f16 multiplies the integer codes, O = sum w_j code_j, L = sum w_j / a_j,
-// o = O / L.  (A page whose V scale is 0 holds zeros only and counts with a = 1.)  w_j's rounding to f16 is the only one
+// o = O / L.  (A page whose V scale is 0 counts with a = 2^-80 in w and L, so that it does not push the others' weights out of
+// f16's range, and its weights are 0 in O.)  w_j's rounding to f16 is the only one
 // besides the final bf16: 2^-12 of w_j, averaged over the tokens; 2^-40 of the largest weight for weights below 2^-29
 // of it, which is what the factor 2^15 is for.
 //
@@ -59,6 +60,7 @@ constexpr int kKvTile = 16;
 constexpr int kKvUnitCost = 32;
 constexpr int kKvMaxBatch = 4096;
 constexpr float kKvTop = 15.f;  // the largest weight is 2^15, the top of f16's range
+constexpr float kKvNone = 0x1p-80f;  // in place of a V scale of 0: below real ones, and its reciprocal times 2^15 far from fp32's top
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
@@ -321,7 +323,8 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
           mma_f16_16816(s[nt], a0, a1, a2, a3, q2.x, q2.y);
         }
       }
-      const float ks_now = __uint_as_float(ks), vs_now = vs << 1 == 0 ? 1.f : __uint_as_float(vs);
+      const float ks_now = __uint_as_float(ks), vs_now = vs << 1 == 0 ? kKvNone : __uint_as_float(vs);
+      const bool none = vs << 1 == 0;
       const bool more = next < stop, here = page >= 0;
       page = page_of(entry_next);  // (read a tile ahead; page 0 where there is no next tile)
       const bool loads = more && page >= 0;
@@ -371,6 +374,10 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
         if (w1 + w3 != 0.f) l[nt][1] = fmaf(w1 + w3, inv_v, l[nt][1]);
         pb[nt][0] = movmatrix_trans(pack_f16x2(w0, w1));
         pb[nt][1] = movmatrix_trans(pack_f16x2(w2, w3));
+      }
+      if (none) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) pb[nt][0] = pb[nt][1] = 0;
       }
 #pragma unroll
       for (int j = 0; j < kD / 32; ++j) {

@@ -60,7 +60,7 @@ struct KvTilePlan {
   static constexpr int kRaw = kTileStep * kD;            // bytes of a staged step of codes
   static constexpr int kRing = kD == 128 ? 6 : 12;       // staged steps, K and V in turn: 48 KB
   static constexpr int kVAt = kTileBufs * kOperand, kQAt = 2 * kVAt, kRingAt = kQAt + 2 * kQTile, kCtrlAt = kRingAt + kRing * kRaw;
-  static constexpr int kCtrl = 8176;                     // scales, barriers, small shared state
+  static constexpr int kCtrl = 8304;                     // scales, barriers, small shared state
   static constexpr int smem(int B) { return 1024 + kCtrlAt + kCtrl + (B + 1) * 4; }
   // Tensor memory columns of stream s: its two S (the f16 weights over their S), O.
   __host__ __device__ static constexpr uint32_t s_at(int s, int buf) { return 128u * s + 64u * buf; }
@@ -69,7 +69,9 @@ struct KvTilePlan {
 };
 
 struct KvTileCtrl {
-  alignas(16) float scale_k[8][4], lv[8][4], inv_v[8][4];  // by step % 8 and group of 16 tokens
+  // By step % 8 and group of 16 tokens.  A V scale of 0 has mul 0 and turns the sign of inv_v[0] or [2]: the softmax threads take
+  // two groups each and look at the first one's sign alone.
+  alignas(16) float scale_k[8][4], lv[8][4], inv_v[8][4], mul[8][4];
   uint64_t k_full[kTileBufs], k_empty[kTileBufs], v_full[kTileBufs], v_empty[kTileBufs], raw_full[12], raw_empty[12];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full[2], q_free;  // [stream][item % 2]: an item is a stream's step
   uint32_t tmem;
@@ -78,7 +80,7 @@ struct KvTileCtrl {
   float swap[2][2][2][kTileRows];  // [maxima of items, else][stream][half][row]: what a row's two threads tell each other
   float row_scale[2][2][kTileRows];  // [unit % 2][row tile][row]: of the scores
 };
-static_assert(sizeof(KvTileCtrl) <= 8176, "control block");
+static_assert(sizeof(KvTileCtrl) <= 8304, "control block");
 
 // The token tiles of the 256-row unit rt of a sequence: t0 .. t1 - 1.
 __device__ __forceinline__ void kv_tile_range(const KvAttnArgs& a, const KvSpan& s, int rt, int& t0, int& t1) {
@@ -439,12 +441,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       for (; st < st_end; ++st, ++steps) {
         const uint32_t buf = steps % kTileBufs, use = steps / kTileBufs;
         if (use > 0) tile_wait(&ct->k_empty[buf], use - 1, dead);
+        const bool none = scale << 1 == 0;
+        const uint32_t marked = __ballot_sync(0xffffffffu, none);
         if (lane < 4) {
           ct->scale_k[steps & 7][lane] = __uint_as_float(scale);
         } else if (lane < 8) {
-          const float sv = scale << 1 == 0 ? 1.f : __uint_as_float(scale);
+          const float sv = none ? kKvNone : __uint_as_float(scale), inv = __fdividef(1.f, sv);
           ct->lv[steps & 7][lane & 3] = here ? lg2(sv) : -INFINITY;
-          ct->inv_v[steps & 7][lane & 3] = __fdividef(1.f, sv);
+          ct->inv_v[steps & 7][lane & 3] = (lane & 1) == 0 && (marked >> lane & 3) != 0 ? -inv : inv;
+          ct->mul[steps & 7][lane & 3] = none ? 0.f : 1.f;
         }
         scale = scale_of(entry_next);
         here = entry_next < a.c.pages;
@@ -647,10 +652,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
               sum = add_f32x2(sum, pack_f32x2(w0, w1));
               w[k * 8 + j / 2] = pack_f16x2(w0, w1);
             }
-            if (!cut || bits >> (16 * k) & 0xFFFFu) l = fmaf(unpack_f32x2(sum).x + unpack_f32x2(sum).y, iv[k], l);  // (a hidden page's scale may be anything)
+            if (!cut || bits >> (16 * k) & 0xFFFFu) l = fmaf(unpack_f32x2(sum).x + unpack_f32x2(sum).y, k == 0 ? fabsf(iv[k]) : iv[k], l);  // (a hidden page's scale may be anything)
           }
         };
         if (whole) weights(std::false_type{}); else weights(std::true_type{});
+        if (iv[0] < 0.f) {  // a page whose V scale is 0 adds nothing to O
+          const float2 mul = *reinterpret_cast<const float2*>(&ct->mul[sl][g0]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = (i < 8 ? mul.x : mul.y) == 0.f ? 0u : w[i];
+        }
         tmem_st16(ts + half * 16, w);
         tmem_wait_st();
         tc_fence_before();

@@ -142,3 +142,20 @@ def test_pages_outside_the_cache_are_skipped(cuda, form, page):
     assert torch.isfinite(ref[0]).all() and (ref[0][2] == 0).all()
     check(out, lse, ref, cache, table, lens)
     assert (out[2] == 0).all()
+
+
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+@pytest.mark.parametrize("log2", [-70, -40, -30, -8, 20])
+def test_pages_of_zeros_beside_pages_of_any_scale(cuda, form, log2):
+    """A page whose V scale is 0 takes its softmax mass and adds nothing, whatever its codes are and however small the other
+    pages' values are."""
+    R = form[1]
+    lens = [R + 150, R + 40]
+
+    def edit(c, table):
+        c[3].mul_(64 * 2.0 ** log2)
+        for b in range(2):
+            c[3][table[b, ::2].long()] = 0
+
+    out, lse, ref, cache, table = call(cuda, form, lens, edit=edit, seed=4)
+    check(out, lse, ref, cache, table, lens)
