@@ -9,10 +9,11 @@
 // running maximum, the sum and the output accumulators are fp32.  With s_j the base-2 logit and a_j the V scale of
 // token j's page, the kernel keeps m = max_j (s_j + log2 a_j) and w_j = 2^(s_j + log2 a_j - m + 15) <= 2^15: the page
 // scale of V is part of the exponent, so w_j in f16 multiplies the integer codes, O = sum w_j code_j, L = sum w_j / a_j,
-// o = O / L.  (A page whose V scale is 0 counts with a = 2^-80 in w and L, so that it does not push the others' weights out of
-// f16's range, and its weights are 0 in O.)  w_j's rounding to f16 is the only one
+// o = O / L.  L is kept times 2^-20: for V scales from 2^-112 to 2^106 neither it nor 2^-20 / a_j leaves fp32's normal numbers.
+// A smaller scale counts as 2^-112 in w and L (0 as 2^-80, so that it does not push the others' weights out of f16's range),
+// and its weights are multiplied by what is missing (0) for O.  w_j's rounding to f16 is the only one
 // besides the final bf16: 2^-12 of w_j, averaged over the tokens; 2^-40 of the largest weight for weights below 2^-29
-// of it, which is what the factor 2^15 is for.
+// of it, which is what the factor 2^15 is for (2^-26 of it where all V scales are below 2^-112, values below 2.5e-32).
 //
 // Work.  The cache positions of all (sequence, kv head, row tile) units are laid out in one line of 16-token tiles, with a
 // stretch for each unit's own cost before them, and cut into equal slices, one per CTA, whatever the lengths are; lengths
@@ -60,7 +61,8 @@ constexpr int kKvTile = 16;
 constexpr int kKvUnitCost = 32;
 constexpr int kKvMaxBatch = 4096;
 constexpr float kKvTop = 15.f;  // the largest weight is 2^15, the top of f16's range
-constexpr float kKvNone = 0x1p-80f;  // in place of a V scale of 0: below real ones, and its reciprocal times 2^15 far from fp32's top
+constexpr float kKvNone = 0x1p-80f, kKvLeast = 0x1p-112f;  // V scales in w and L: in place of 0, and the least
+constexpr float kKvSum = 0x1p-20f, kKvSumLog2 = -20.f;      // of L
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
@@ -77,6 +79,10 @@ __device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t hmul2_u32(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 // f16 pairs of bytes 0, 1 and of bytes 2, 3 of u (code + 128): 0x6400 | u is 1024 + u, less 1152.
 __device__ __forceinline__ uint32_t codes_lo_f16x2(uint32_t u) { return hsub2_u32(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u); }
 __device__ __forceinline__ uint32_t codes_hi_f16x2(uint32_t u) { return hsub2_u32(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u); }
@@ -90,9 +96,17 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What stands for the V scale v in w and L (NaN: the least), and its log2: NaN where v is not finite, so that every logit of
+// the page is.
+__device__ __forceinline__ float kv_counts_as(float v) { return v == 0.f ? kKvNone : fmaxf(v, kKvLeast); }
+__device__ __forceinline__ float kv_log2(float v, float counts) { return fmaf(v, 0.f, lg2(counts)); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t scale_f16x2(uint32_t w, float by) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pack_f16x2(f.x * by, f.y * by);
 }
 
 // kBytes consecutive bytes (4, 8 or 16 at a time) of a cache page into words (predicated as ld_cg32_if); read
@@ -323,8 +337,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
           mma_f16_16816(s[nt], a0, a1, a2, a3, q2.x, q2.y);
         }
       }
-      const float ks_now = __uint_as_float(ks), vs_now = vs << 1 == 0 ? kKvNone : __uint_as_float(vs);
-      const bool none = vs << 1 == 0;
+      const float ks_now = __uint_as_float(ks), vs_now = __uint_as_float(vs);
       const bool more = next < stop, here = page >= 0;
       page = page_of(entry_next);  // (read a tile ahead; page 0 where there is no next tile)
       const bool loads = more && page >= 0;
@@ -332,7 +345,8 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
       entry_next = more ? entry_next : 0;
       ld_cg32_if(entry_next, table + (((next + kKvWarps) * kKvTile) >> lg), next + kKvWarps < stop);
 
-      const float lv = lg2(vs_now), inv_v = __fdividef(1.0f, vs_now);
+      // (the reciprocal is finite whatever the page's scale is: a row that the mask hides from the page adds 0 times it)
+      const float av = kv_counts_as(vs_now), lv = kv_log2(vs_now, av), inv_v = __fdividef(kKvSum, av);
       const int p0 = tile * kKvTile;
       const bool whole = p0 >= all_lo && p0 + kKvTile <= all_hi && here;
       uint32_t pb[kNT][2];
@@ -369,15 +383,15 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
         }
         const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] - kKvTop, m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] - kKvTop;
         const float w0 = ex2(x[0] - m0), w1 = ex2(x[1] - m1), w2 = ex2(x[2] - m0), w3 = ex2(x[3] - m1);
-        // (a row that sees none of the tile adds nothing: the page's scale may be anything there, and its weights are 0)
-        if (w0 + w2 != 0.f) l[nt][0] = fmaf(w0 + w2, inv_v, l[nt][0]);
-        if (w1 + w3 != 0.f) l[nt][1] = fmaf(w1 + w3, inv_v, l[nt][1]);
+        l[nt][0] = fmaf(w0 + w2, inv_v, l[nt][0]);
+        l[nt][1] = fmaf(w1 + w3, inv_v, l[nt][1]);
         pb[nt][0] = movmatrix_trans(pack_f16x2(w0, w1));
         pb[nt][1] = movmatrix_trans(pack_f16x2(w2, w3));
       }
-      if (none) {
+      if (vs_now < kKvLeast) {
+        const float by = vs_now * (1.f / kKvLeast);
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) pb[nt][0] = pb[nt][1] = 0;
+        for (int nt = 0; nt < kNT; ++nt) pb[nt][0] = scale_f16x2(pb[nt][0], by), pb[nt][1] = scale_f16x2(pb[nt][1], by);
       }
 #pragma unroll
       for (int j = 0; j < kD / 32; ++j) {
@@ -426,8 +440,8 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
       const bool some = r < sp.n;
       const float inv = some ? (sum == 0.f ? 0.f : 1.0f / sum) : 0.f;
       const int64_t row = (static_cast<int64_t>(b) * a.R + r) * a.heads + h * a.group + rr % a.group;
-      *reinterpret_cast<uint32_t*>(a.o + row * kD + d) = some ? pack_bf16x2(v0 * inv, v1 * inv) : 0u;
-      if (a.lse && d == 0) a.lse[row] = some && sum != 0.f ? (mx - kKvTop + lg2(sum)) * 0.69314718055994531f : -INFINITY;
+      *reinterpret_cast<uint32_t*>(a.o + row * kD + d) = some ? pack_bf16x2(v0 * kKvSum * inv, v1 * kKvSum * inv) : 0u;
+      if (a.lse && d == 0) a.lse[row] = some && sum != 0.f ? (mx - kKvTop - kKvSumLog2 + lg2(sum)) * 0.69314718055994531f : -INFINITY;
     };
     for (int f = warp; f < P::kFrags; f += kKvWarps) {
       const int nt = f / P::kSteps, i = f % P::kSteps, n = nt * 8 + 2 * t;

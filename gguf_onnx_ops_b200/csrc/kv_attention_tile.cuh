@@ -1,7 +1,7 @@
 // Attention of many query rows over the 8-bit paged KV cache: 128-row tiles on tcgen05 (the formulas, the scaling of q
 // and the use of V's page scale are those of kv_attention.cuh; w_j <= 2^15 here too, kept so by a running maximum that moves
 // only when it has grown by more than 2^4, with weights scaled to 2^11: f16 rounds a weight by 2^-12 of it, or by 2^-36 of the
-// largest for weights below 2^-25 of it).
+// largest for weights below 2^-25 of it, 2^-22 where all V scales are below 2^-112).
 //
 // Why.  R * heads / kv_heads rows share the K and V of a kv head.  The streaming kernel converts the codes once per 16
 // rows and multiplies on mma.sync; from 17 rows on that work, not the bytes, is its time (48 rows, 16 sequences of 801 to 9001
@@ -69,9 +69,10 @@ struct KvTilePlan {
 };
 
 struct KvTileCtrl {
-  // By step % 8 and group of 16 tokens.  A V scale of 0 has mul 0 and turns the sign of inv_v[0] or [2]: the softmax threads take
-  // two groups each and look at the first one's sign alone.
-  alignas(16) float scale_k[8][4], lv[8][4], inv_v[8][4], mul[8][4];
+  // By step % 8 and group of 16 tokens.  A V scale below kKvLeast turns the sign of inv_v[0] or [2] (the softmax threads take two
+  // groups each and look at the first one's sign alone); weights are then multiplied by mul (f16 twice, a power of two or 0).
+  alignas(16) float scale_k[8][4], lv[8][4], inv_v[8][4];
+  uint32_t mul[8][4];
   uint64_t k_full[kTileBufs], k_empty[kTileBufs], v_full[kTileBufs], v_empty[kTileBufs], raw_full[12], raw_empty[12];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full[2], q_free;  // [stream][item % 2]: an item is a stream's step
   uint32_t tmem;
@@ -441,15 +442,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       for (; st < st_end; ++st, ++steps) {
         const uint32_t buf = steps % kTileBufs, use = steps / kTileBufs;
         if (use > 0) tile_wait(&ct->k_empty[buf], use - 1, dead);
-        const bool none = scale << 1 == 0;
-        const uint32_t marked = __ballot_sync(0xffffffffu, none);
+        const float sv = __uint_as_float(scale);
+        const uint32_t faint = __ballot_sync(0xffffffffu, sv < kKvLeast);
         if (lane < 4) {
-          ct->scale_k[steps & 7][lane] = __uint_as_float(scale);
+          ct->scale_k[steps & 7][lane] = sv;
         } else if (lane < 8) {
-          const float sv = none ? kKvNone : __uint_as_float(scale), inv = __fdividef(1.f, sv);
-          ct->lv[steps & 7][lane & 3] = here ? lg2(sv) : -INFINITY;
-          ct->inv_v[steps & 7][lane & 3] = (lane & 1) == 0 && (marked >> lane & 3) != 0 ? -inv : inv;
-          ct->mul[steps & 7][lane & 3] = none ? 0.f : 1.f;
+          float av = kv_counts_as(sv), mul = 1.f;
+          if (sv < kKvLeast) {  // its bits with kKvLeast's exponent, and the power of two that is missing
+            const int up = -112 - (static_cast<int>(__float_as_uint(sv * 0x1p60f) >> 23) - 127 - 60);
+            mul = sv == 0.f ? 0.f : pow2i(-up);
+            if (sv != 0.f) av = sv * pow2i(up);
+          }
+          const float inv = __fdividef(kKvSum, av);
+          ct->lv[steps & 7][lane & 3] = here ? kv_log2(sv, av) : -INFINITY;
+          ct->inv_v[steps & 7][lane & 3] = (lane & 1) == 0 && (faint >> lane & 3) != 0 ? -inv : inv;
+          ct->mul[steps & 7][lane & 3] = pack_f16x2(mul, mul);
         }
         scale = scale_of(entry_next);
         here = entry_next < a.c.pages;
@@ -652,14 +659,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
               sum = add_f32x2(sum, pack_f32x2(w0, w1));
               w[k * 8 + j / 2] = pack_f16x2(w0, w1);
             }
-            if (!cut || bits >> (16 * k) & 0xFFFFu) l = fmaf(unpack_f32x2(sum).x + unpack_f32x2(sum).y, k == 0 ? fabsf(iv[k]) : iv[k], l);  // (a hidden page's scale may be anything)
+            if (!cut || bits >> (16 * k) & 0xFFFFu) l = fmaf(unpack_f32x2(sum).x + unpack_f32x2(sum).y, k == 0 ? fabsf(iv[k]) : iv[k], l);
           }
         };
         if (whole) weights(std::false_type{}); else weights(std::true_type{});
-        if (iv[0] < 0.f) {  // a page whose V scale is 0 adds nothing to O
-          const float2 mul = *reinterpret_cast<const float2*>(&ct->mul[sl][g0]);
+        if (iv[0] < 0.f) {
+          const uint2 mul = *reinterpret_cast<const uint2*>(&ct->mul[sl][g0]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = (i < 8 ? mul.x : mul.y) == 0.f ? 0u : w[i];
+          for (int i = 0; i < 16; ++i) w[i] = hmul2_u32(w[i], i < 8 ? mul.x : mul.y);
         }
         tmem_st16(ts + half * 16, w);
         tmem_wait_st();
@@ -692,7 +699,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
       }
       if (!(joins && s == 1)) {
         const int64_t out_row = out_row_of();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // (kKvSum is taken out of the other factor: 1 / l may be large)
         const int64_t slot = kv_tile_slot(blockIdx.x, u.ta == 0, s);
 #pragma unroll 1
         for (int c = 0; c < kD / 32; ++c) {
@@ -718,15 +725,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
               uint2* o = reinterpret_cast<uint2*>(a.o + out_row * kD + half * (kD / 2) + c * 16);
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                o[i] = on ? make_uint2(pack_bf16x2(__uint_as_float(x[4 * i]) * inv, __uint_as_float(x[4 * i + 1]) * inv),
-                                       pack_bf16x2(__uint_as_float(x[4 * i + 2]) * inv, __uint_as_float(x[4 * i + 3]) * inv))
+                o[i] = on ? make_uint2(pack_bf16x2(__uint_as_float(x[4 * i]) * kKvSum * inv, __uint_as_float(x[4 * i + 1]) * kKvSum * inv),
+                                       pack_bf16x2(__uint_as_float(x[4 * i + 2]) * kKvSum * inv, __uint_as_float(x[4 * i + 3]) * kKvSum * inv))
                           : make_uint2(0u, 0u);
             }
           }
         }
         if (half == 0) {
           if (cut_unit) __stcg(a.ml + slot * kTileRows + row, make_float2(m, l));
-          else if (exists && a.lse) a.lse[out_row] = on && l != 0.f ? (m - kTileTop + lg2(l)) * 0.69314718055994531f : -INFINITY;
+          else if (exists && a.lse) a.lse[out_row] = on && l != 0.f ? (m - kTileTop - kKvSumLog2 + lg2(l)) * 0.69314718055994531f : -INFINITY;
         }
       }
       tc_fence_before();
@@ -831,8 +838,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t out_row = (static_cast<int64_t>(b) * a.R + r) * a.heads + h * a.group + rr % a.group;
     reinterpret_cast<uint2*>(a.o + out_row * kD)[c] =
-        on ? make_uint2(pack_bf16x2(acc[j].x * inv, acc[j].y * inv), pack_bf16x2(acc[j].z * inv, acc[j].w * inv)) : make_uint2(0u, 0u);
-    if (a.lse && c == 0) a.lse[out_row] = on && sum != 0.f ? (part_ml[0][row].x - kTileTop + lg2(sum)) * 0.69314718055994531f : -INFINITY;
+        on ? make_uint2(pack_bf16x2(acc[j].x * kKvSum * inv, acc[j].y * kKvSum * inv), pack_bf16x2(acc[j].z * kKvSum * inv, acc[j].w * kKvSum * inv))
+           : make_uint2(0u, 0u);
+    if (a.lse && c == 0) a.lse[out_row] = on && sum != 0.f ? (part_ml[0][row].x - kTileTop - kKvSumLog2 + lg2(sum)) * 0.69314718055994531f : -INFINITY;
   }
 }
 

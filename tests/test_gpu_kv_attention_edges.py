@@ -159,3 +159,16 @@ def test_pages_of_zeros_beside_pages_of_any_scale(cuda, form, log2):
 
     out, lse, ref, cache, table = call(cuda, form, lens, edit=edit, seed=4)
     check(out, lse, ref, cache, table, lens)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+@pytest.mark.parametrize("scale", [3e-38, 1e-36, 1e-33, 1e-30, 1e25, 1e33])
+def test_values_of_any_size(cuda, form, scale):
+    """V scales over the range of what KvCacheWrite makes: tiny values keep their softmax and its sum."""
+    lens = [form[1] + 900, form[1] + 3]
+
+    def edit(c, table):
+        c[3].mul_(64 * scale / 2)
+
+    out, lse, ref, cache, table = call(cuda, form, lens, edit=edit, seed=5)
+    check(out, lse, ref, cache, table, lens)
