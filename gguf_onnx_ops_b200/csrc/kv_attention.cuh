@@ -100,6 +100,8 @@ __device__ __forceinline__ float lg2(float x) {
 // the page is.
 __device__ __forceinline__ float kv_counts_as(float v) { return v == 0.f ? kKvNone : fmaxf(v, kKvLeast); }
 __device__ __forceinline__ float kv_log2(float v, float counts) { return fmaf(v, 0.f, lg2(counts)); }
+// A K scale, NaN where it is not finite (an infinite one would make -inf of a negative score, and hide its token).
+__device__ __forceinline__ float kv_finite(float k) { return fmaf(k, 0.f, k); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(kKvThreads, KvAttnPlan<kD, kNT>::kCtas) kv_att
           mma_f16_16816(s[nt], a0, a1, a2, a3, q2.x, q2.y);
         }
       }
-      const float ks_now = __uint_as_float(ks), vs_now = __uint_as_float(vs);
+      const float ks_now = kv_finite(__uint_as_float(ks)), vs_now = __uint_as_float(vs);
       const bool more = next < stop, here = page >= 0;
       page = page_of(entry_next);  // (read a tile ahead; page 0 where there is no next tile)
       const bool loads = more && page >= 0;

@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_attention_tile_kernel(cons
         const float sv = __uint_as_float(scale);
         const uint32_t faint = __ballot_sync(0xffffffffu, sv < kKvLeast);
         if (lane < 4) {
-          ct->scale_k[steps & 7][lane] = sv;
+          ct->scale_k[steps & 7][lane] = kv_finite(sv);
         } else if (lane < 8) {
           float av = kv_counts_as(sv), mul = 1.f;
           if (sv < kKvLeast) {  // its bits with kKvLeast's exponent, and the power of two that is missing

@@ -86,7 +86,7 @@ def check(out, lse, ref, cache, table, lens, where=None):
 
 @pytest.mark.parametrize("form", FORMS, ids=IDS)
 @pytest.mark.parametrize("which", ["k", "v", "both"])
-@pytest.mark.parametrize("bad", [float("nan")])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_a_marked_page_reaches_only_rows_that_see_it(cuda, form, which, bad):
     """The last token begins a page whose scale is not finite: the rows before it are what they are without that page."""
     R, page = form[1], 16
