@@ -59,6 +59,15 @@ def _raw_stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+def _current_device() -> int:
+    """The device that launches go to, for tensors that are on one (torch.cuda.current_device, but for its initialisation)."""
+    return torch._C._cuda_getDevice()
+
+
+def _wrong_device(t, name: str, op: str) -> ValueError:
+    return ValueError(f"{op}: tensors must be on one device" if t.is_cuda else f"{op}: {name} must be a CUDA tensor")
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -68,6 +77,18 @@ def _need(t, name, dtype, op):
         raise ValueError(f"{op}: Missing required tensor input {name}")
     if not t.is_cuda:
         raise ValueError(f"{op}: {name} must be a CUDA tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{op}: {name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{op}: {name} must be contiguous")
+
+
+def _need_on(dev: int, t, name, dtype, op):
+    """_need of a tensor on the device of the call's first one."""
+    if t is None:
+        raise ValueError(f"{op}: Missing required tensor input {name}")
+    if t.get_device() != dev:
+        raise _wrong_device(t, name, op)
     if t.dtype != dtype:
         raise ValueError(f"{op}: {name} must be {dtype}, got {t.dtype}")
     if not t.is_contiguous():
@@ -511,7 +532,8 @@ def QkNormRope(qkv: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.T
     them); the first rot values of a head turn as pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved.  Returns
     (q [..., heads, head_dim], k [..., kv_heads, head_dim]); a position outside the tables uses row 0 and is reported by
     device_status()."""
-    if not qkv.is_cuda:
+    dev = qkv.get_device()
+    if dev < 0:
         raise ValueError("QkNormRope: qkv must be a CUDA tensor")
     if qkv.dtype != torch.bfloat16:
         raise ValueError(f"QkNormRope: qkv must be {torch.bfloat16}, got {qkv.dtype}")
@@ -525,16 +547,20 @@ def QkNormRope(qkv: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.T
     if heads < 1 or kv_heads < 1 or width % (heads + 2 * kv_heads) != 0:
         raise ValueError("QkNormRope: qkv width must be (heads + 2 * kv_heads) * head_dim")
     D = width // (heads + 2 * kv_heads)
-    _need(cos, "cos", torch.float32, "QkNormRope")
-    _need(sin, "sin", torch.float32, "QkNormRope")
-    _need(positions, "positions", torch.int32, "QkNormRope")
+    _need_on(dev, cos, "cos", torch.float32, "QkNormRope")
+    _need_on(dev, sin, "sin", torch.float32, "QkNormRope")
+    _need_on(dev, positions, "positions", torch.int32, "QkNormRope")
     if cos.dim() != 2 or cos.shape != sin.shape or positions.numel() != T:
         raise ValueError("QkNormRope: needs cos and sin [max_pos, rot / 2] and one position per row")
     for t, n in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
         if t is not None:
-            _need(t, n, torch.float32, "QkNormRope")
+            _need_on(dev, t, n, torch.float32, "QkNormRope")
             if t.numel() != D:
                 raise ValueError(f"QkNormRope: {n} size mismatch")
+    if dev != _current_device():  # launches go there
+        with torch.cuda.device(dev):
+            return QkNormRope(qkv, q_gamma, k_gamma, cos, sin, positions, heads=heads, kv_heads=kv_heads, epsilon=epsilon,
+                              interleaved=interleaved)
     lead = qkv.shape[:-1]
     q = qkv.new_empty((*lead, heads, D))
     k = qkv.new_empty((*lead, kv_heads, D))
@@ -547,7 +573,7 @@ class KvCache:
     """The paged 8-bit cache of one attention layer: int8 codes k, v [pages, kv_heads, page, head_dim] and one f32 scale for
     each page and head, k_scale, v_scale [pages, kv_heads]; a value is code * scale."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "_c", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "device_index", "_c", "_ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         for t, n, dt in ((k, "k", torch.int8), (v, "v", torch.int8), (k_scale, "k_scale", torch.float32),
@@ -558,6 +584,7 @@ class KvCache:
         if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
             raise ValueError("KvCache: tensors must be on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device_index = k.get_device()
         self.pages, self.kv_heads, self.page, self.head_dim = k.shape
         if self.page not in (16, 32, 64, 128, 256):
             raise ValueError("KvCache: page must be 16, 32, 64, 128 or 256 tokens")
@@ -576,22 +603,24 @@ class KvCache:
 
 
 def _kv_batch(op, cache, page_table, lens, new_lens):
-    _need(page_table, "page_table", torch.int32, op)
-    _need(lens, "lens", torch.int32, op)
+    dev = cache.device_index
+    _need_on(dev, page_table, "page_table", torch.int32, op)
+    _need_on(dev, lens, "lens", torch.int32, op)
     B = lens.shape[0] if lens.dim() == 1 else -1
     if page_table.dim() != 2 or page_table.shape[0] != B:
         raise ValueError(f"{op}: needs page_table [B, pages of a sequence] and lens [B]")
     if new_lens is not None:
-        _need(new_lens, "new_lens", torch.int32, op)
+        _need_on(dev, new_lens, "new_lens", torch.int32, op)
         if new_lens.shape != lens.shape:
             raise ValueError(f"{op}: new_lens must have one number per sequence")
     return B, page_table.shape[1]
 
 
-def _kv_rows(op, name, t, B, heads, D):
+def _kv_rows(op, name, t, B, heads, cache):
     """The strides of t bf16 [B, R, heads, D] whose [heads, D] block is contiguous."""
-    if not t.is_cuda:
-        raise ValueError(f"{op}: {name} must be a CUDA tensor")
+    D = cache.head_dim
+    if t.get_device() != cache.device_index:
+        raise _wrong_device(t, name, op)
     if t.dtype != torch.bfloat16:
         raise ValueError(f"{op}: {name} must be {torch.bfloat16}, got {t.dtype}")
     if t.dim() != 4 or t.shape[0] != B or (heads and t.shape[2] != heads) or t.shape[3] != D:
@@ -619,10 +648,13 @@ def KvCacheWrite(k: torch.Tensor, v: torch.Tensor, cache: KvCache, page_table: t
     begins the page; code = rint(x * (1 / s')); the page's older codes become rint(code * (s / s')).  A value that is not
     finite makes the scale NaN.  A shorter lens later (a rollback) needs no call; the scale stays."""
     B, cols = _kv_batch("KvCacheWrite", cache, page_table, lens, new_lens)
-    ks = _kv_rows("KvCacheWrite", "k", k, B, cache.kv_heads, cache.head_dim)
-    vs = _kv_rows("KvCacheWrite", "v", v, B, cache.kv_heads, cache.head_dim)
+    ks = _kv_rows("KvCacheWrite", "k", k, B, cache.kv_heads, cache)
+    vs = _kv_rows("KvCacheWrite", "v", v, B, cache.kv_heads, cache)
     if v.shape != k.shape:
         raise ValueError("KvCacheWrite: k and v must have the same shape")
+    if cache.device_index != _current_device():
+        with torch.cuda.device(cache.device_index):
+            return KvCacheWrite(k, v, cache, page_table, lens, new_lens)
     kv_cache_write_into(cache, k, v, page_table, lens, new_lens, B, k.shape[1], cols, ks, vs)
 
 
@@ -639,6 +671,9 @@ def KvCacheRead(cache: KvCache, page_table: torch.Tensor, lens: torch.Tensor, *,
     B, cols = _kv_batch("KvCacheRead", cache, page_table, lens, None)
     if rows < 0:
         raise ValueError("KvCacheRead: rows must be >= 0")
+    if cache.device_index != _current_device():
+        with torch.cuda.device(cache.device_index):
+            return KvCacheRead(cache, page_table, lens, rows=rows)
     k = torch.empty(B, rows, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.k.device)
     v = torch.empty_like(k)
     kv_cache_read_into(cache, page_table, lens, k, v, B, rows, cols)
@@ -715,14 +750,20 @@ def KvCacheAttention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, 
     captured graph's replay on another."""
     op = "KvCacheAttention"
     B, cols = _kv_batch(op, cache, page_table, lens, new_lens)
-    strides = _kv_rows(op, "q", q, B, 0, cache.head_dim)
+    strides = _kv_rows(op, "q", q, B, 0, cache)
     R, heads = q.shape[1], q.shape[2]
     if heads == 0 or heads % cache.kv_heads != 0:
         raise ValueError(f"{op}: heads must be a multiple of kv heads")
+    if cache.device_index != _current_device():
+        with torch.cuda.device(cache.device_index):
+            return KvCacheAttention(q, cache, page_table, lens, new_lens, scale=scale, window=window, return_lse=return_lse,
+                                    workspace=workspace)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(B, R, heads, dtype=torch.float32, device=q.device) if return_lse else None
     ws = workspace if workspace is not None else _kv_workspace(q.device, _raw_stream(q))
     ws.fit(B, R, heads, cache.kv_heads, cache.head_dim)
+    if ws.scratch.get_device() != cache.device_index:
+        raise _wrong_device(ws.scratch, "workspace", op)
     kv_cache_attention_into(cache, q, page_table, lens, new_lens, out, lse, ws, B, R, heads, cols, strides,
                             cache.head_dim ** -0.5 if scale is None else scale, window)
     return (out, lse) if return_lse else out
@@ -749,9 +790,10 @@ def DraftVerify(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, dr
     accepted[b] is the state_row of the sequence's next MambaVerify."""
     op = "DraftVerify"
     _need(target_probs, "target_probs", torch.float32, op)
-    _need(draft_tokens, "draft_tokens", torch.int32, op)
-    _need(u_accept, "u_accept", torch.float32, op)
-    _need(u_sample, "u_sample", torch.float32, op)
+    dev = target_probs.get_device()
+    _need_on(dev, draft_tokens, "draft_tokens", torch.int32, op)
+    _need_on(dev, u_accept, "u_accept", torch.float32, op)
+    _need_on(dev, u_sample, "u_sample", torch.float32, op)
     if draft_tokens.dim() != 2 or target_probs.dim() != 3:
         raise ValueError(f"{op}: needs target_probs [B, R + 1, V] and draft_tokens [B, R]")
     B, R = draft_tokens.shape
@@ -759,13 +801,16 @@ def DraftVerify(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, dr
     if target_probs.shape[:2] != (B, R + 1) or u_accept.shape != draft_tokens.shape or u_sample.shape != (B,):
         raise ValueError(f"{op}: needs target_probs [B, R + 1, V], u_accept [B, R] and u_sample [B]")
     if draft_probs is not None:
-        _need(draft_probs, "draft_probs", torch.float32, op)
+        _need_on(dev, draft_probs, "draft_probs", torch.float32, op)
         if draft_probs.shape != (B, R, V):
             raise ValueError(f"{op}: draft_probs must be [B, R, V]")
     if drafts is not None:
-        _need(drafts, "drafts", torch.int32, op)
+        _need_on(dev, drafts, "drafts", torch.int32, op)
         if drafts.shape != (B,):
             raise ValueError(f"{op}: drafts must have one number per sequence")
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return DraftVerify(target_probs, draft_probs, draft_tokens, u_accept, u_sample, drafts)
     accepted = draft_tokens.new_empty((B,))
     tokens = draft_tokens.new_empty((B, R + 1))
     draft_verify_into(target_probs, draft_probs, draft_tokens, u_accept, u_sample, drafts, accepted, tokens, B, R, V)
