@@ -315,10 +315,16 @@ int gguf_kv_cache_attention(const GgufKvCache* cache, const void* q, const int32
   if (!q || !out || !workspace || !counters) return invalid(op, "null tensor pointer");
   if (!is_aligned(q, 16) || !is_aligned(out, 16) || !is_aligned(workspace, 16) || q_stride_b % 8 || q_stride_r % 8)
     return invalid(op, "tensors must be 16-byte aligned with strides in multiples of 8 values");
-  int sms = 0;
-  if (int rc = device_sms(&sms)) return rc;
   const int64_t group = heads / cache->kv_heads, rows = R * group;
   const int64_t width = table_cols << a.c.log2_page, positions = window > 0 ? std::min(width, window + R) : width;
+  if (rows >= (1ll << 31)) return invalid(op, "too many rows");
+  // The kernels sum the line's tiles of all sequences (the tile kernel: of all their row tiles) in 32 bits.
+  const int64_t line = B * (positions / kKvTile + 2 + kKvUnitCost);
+  const int64_t tile_line = B * ((rows + kTileUnitRows - 1) / kTileUnitRows) * (positions / kTileTokens + 2 + kTileUnitCost);
+  if (line >= (1ll << 31) || (tile_rows(B, rows, cache->head_dim) && tile_line >= (1ll << 31)))
+    return invalid(op, "too many positions in all (a narrower page table, or fewer sequences or rows a call)");
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
   const AttentionPlan p = attention_plan(B, rows, cache->head_dim, cache->kv_heads, positions, sms);
   if (B * cache->kv_heads * p.row_tiles >= (1ll << 31)) return invalid(op, "too many rows");
   a.k = static_cast<const int8_t*>(cache->k), a.v = static_cast<const int8_t*>(cache->v);

@@ -341,7 +341,8 @@ GGUF_OPS_API int gguf_kv_cache_read(const GgufKvCache* cache, const int32_t* tab
  * max(0, t - window + 1) .. t (window 0: 0 .. t); its output is sum_j softmax_j(scale q.k_j) v_j.  Rows r >= n give 0 (lse
  * -inf).  workspace and counters have the sizes that gguf_kv_cache_attention_workspace gives for the current device;
  * counters must be zero before the first call and are left zero.  Calls that may overlap need workspaces of their own.
- * Contract: B <= 4096.
+ * Contract: B <= 4096; the positions that the table has room for, over all sequences (and, for many rows, row tiles of 256),
+ * fit 32 bits in tiles of 16 (128): any real call.
  */
 GGUF_OPS_API int gguf_kv_cache_attention_workspace(int64_t B, int64_t R, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                    int64_t* bytes, int64_t* counters);

@@ -77,6 +77,14 @@ def test_attention(lib):
     refused(lib, "gguf_kv_cache_attention_workspace", (1, 1, 4, 2, 128, None, ctypes.byref(n)), "null")
 
 
+@pytest.mark.parametrize("page,cols,B,R,heads", [(256, 1 << 22, 4096, 1, 4), (64, 1 << 14, 8, 1 << 20, 32), (64, 4, 1, 1 << 24, 512)])
+def test_attention_of_more_than_32_bits_count(lib, page, cols, B, R, heads):
+    """Page tables and rows whose tiles, summed over the call, would pass 32 bits."""
+    kc = cache(page=page)
+    refused(lib, "gguf_kv_cache_attention", (ctypes.addressof(kc), FAKE, FAKE, FAKE, None, FAKE, None, FAKE, FAKE, B, R, heads, cols,
+                                             512, 512, 0.1, 0, None), "too many")
+
+
 def test_draft(lib):
     args = [FAKE] * 5 + [None, FAKE, FAKE, 2, 3, 1000, None]
     for i, v, msg in ((9, 0, "[1, 32]"), (9, 33, "[1, 32]"), (10, 0, "vocabulary"), (10, (1 << 24) + 1, "vocabulary"), (8, -1, "batch"),
