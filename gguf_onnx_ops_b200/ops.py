@@ -571,7 +571,7 @@ def QkNormRope(qkv: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.T
 
 class KvCache:
     """The paged 8-bit cache of one attention layer: int8 codes k, v [pages, kv_heads, page, head_dim] and one f32 scale for
-    each page and head, k_scale, v_scale [pages, kv_heads]; a value is code * scale."""
+    each page and head, k_scale, v_scale [pages, kv_heads], not negative; a value is code * scale."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page", "head_dim", "device_index", "_c", "_ref")
 

@@ -300,9 +300,11 @@ GGUF_OPS_API int gguf_qk_norm_rope(const void* x, const float* gamma_q, const fl
 
 /*
  * The paged 8-bit KV cache: int8 codes [pages, kv_heads, page, head_dim] for K and for V, and one f32 scale for each page
- * and head [pages, kv_heads]; a value is code * scale.  table i32 [B, table_cols] names the page of each sequence's i-th
- * stretch of `page` tokens; lens i32 [B] is each sequence's length, a call's new tokens included (they are its last
- * n: n = new_lens[b], or R where new_lens is NULL, never more than lens[b]).
+ * and head [pages, kv_heads]; a value is code * scale.  Scales are not negative (KvCacheWrite makes none); a scale that is not
+ * finite marks its page and head: attention rows that see it are NaN, their lse too, and no others.
+ * table i32 [B, table_cols] names the page of each sequence's i-th stretch of `page` tokens; lens i32 [B] is each sequence's
+ * length, a call's new tokens included (they are its last n: n = new_lens[b], or R where new_lens is NULL, never more than
+ * lens[b]).
  * Contract: head_dim 64, 96, 128, 192 or 256; page 16, 32, 64, 128 or 256; codes 16-byte aligned.  A page number or a
  * length outside the cache is skipped (its positions are not written, are read as 0 and are hidden from attention) and
  * reported through gguf_device_status.
