@@ -10,8 +10,9 @@
 // One cluster of up to eight CTAs per sequence: each sums its part of the row (two fp32 reads a token, nothing kept), the
 // CTAs' totals meet through distributed shared memory, and the one warp whose stretch holds the target reads that stretch
 // again (from the L2) to find the token.  Bound by memory for batches and by the chain of cluster barriers for one sequence
-// (64 sequences of 7 drafts and 131072 tokens: 18 us, 3.7 TB/s; one of 5 drafts and 32000 tokens: 5 us, of which a kernel that
-// does nothing takes 2).
+// (64 sequences of 7 drafts and 131072 tokens: 18 us, 3.7 TB/s, 13.4 where the L2 still holds the rows; one of 5 drafts and
+// 32000 tokens: 5 us, of which a kernel that does nothing takes 2).  Rows that do not begin at 16 bytes are read 4 bytes a lane: 64
+// sequences of 50257 tokens 14.9 us, of 50256 tokens 9.4.
 #pragma once
 
 #include <cooperative_groups.h>

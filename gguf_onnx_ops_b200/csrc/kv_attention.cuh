@@ -21,9 +21,13 @@
 // the unit; a unit cut between CTAs leaves its pieces in the workspace, and the CTA that finishes last (a counter per
 // unit) joins them in order, so results do not depend on timing.
 //
-// Bound.  Memory for many sequences (64 of 131 to 8009 tokens, 8 kv heads of 128: 99 us, 5.4 TB/s); for one of 131071
-// tokens the conversion of the codes shares it (57 us, 4.7 TB/s; the ALU pipe 52 % busy); few tokens are a chain of loads
-// (lens, table, page, rows, pieces: 10 us for 777 tokens).  16 rows take half as long again as 8 (85 us against 57).
+// Bound.  Memory for many sequences (64 of 131 to 8009 tokens, 8 kv heads of 128: 101 us one call after the other, 5.3 TB/s;
+// 111 us by itself, when nothing fills the ragged end).  For one of 131071 tokens (58 us, 4.7 TB/s) no unit is full (issue
+// slots 49 %, ALU pipe 46 % busy): with one tile ahead, a warp's loads and its 390 instructions a tile take turns.  Few tokens
+// are a chain of loads (lens, table, page, rows, pieces: 10 us for 777 tokens).  16 rows take half as long again as 8 (85 us
+// against 57).  Other widths, 16 sequences of 801 to 9001 tokens, 8 rows a kv head, in us and of the bytes' time: 96 values 36
+// (1.9x), 128 57 (2.3x), 192 62 (1.7x), 256 67 (1.4x).  Many rows of 96, 192 and 256 values are taken 16 at a time too: a chunk of
+// 128 tokens, 64 heads over 8 kv heads, 9001 positions 254 / 386 / 492 us (96 / 192 / 256).
 //
 // A tile's fragments: S^T (16 tokens x 8 rows) = K (A operand) q^T (B), so that K goes straight from global memory
 // into the A fragment: lane (g, t) loads 16 consecutive bytes of rows g and g + 8, and the order of the head's values
@@ -57,7 +61,8 @@ constexpr int kKvWarps = 8;
 constexpr int kKvThreads = kKvWarps * 32;
 constexpr int kKvTile = 16;
 // What a unit costs besides its tiles (rows read, warps joined, a result written), in tiles: the slices count it, or the CTAs
-// that meet many short sequences end last (64 sequences of 131 to 8009 tokens: 129 us without, 119 with 6, 101 with 24).
+// that meet many short sequences end last (64 sequences of 131 to 8009 tokens, 8 rows of 128 values: 129 us without, 119 with 6,
+// 101 with 24; the other widths use the same number, which was not measured for them).
 constexpr int kKvUnitCost = 32;
 constexpr int kKvMaxBatch = 4096;
 constexpr float kKvTop = 15.f;  // the largest weight is 2^15, the top of f16's range

@@ -5,7 +5,7 @@
 //
 // Why.  R * heads / kv_heads rows share the K and V of a kv head.  The streaming kernel converts the codes once per 16
 // rows and multiplies on mma.sync; from 17 rows on that work, not the bytes, is its time (48 rows, 16 sequences of 801 to 9001
-// tokens: 142 us for 25 us of bytes, 79 us here).  Here a CTA converts each 128-token tile of codes once, to f16 in shared
+// tokens: 144 us for 25 us of bytes, 79 us here).  Here a CTA converts each 128-token tile of codes once, to f16 in shared
 // memory, for up to 256 rows, and the products run on the 5th-generation tensor cores.
 //
 // One CTA per SM, seven warp groups; the tokens go by in steps of 64:
@@ -21,8 +21,8 @@
 // one row tile against every second step when it has one (two accumulators, joined at the end).
 // The line of all units' 128-token tiles is cut into equal slices as in the streaming kernel; a second kernel joins the pieces.
 //
-// Bound.  A step of two streams takes about 2300 cycles: the softmax warps' instructions (issue slots 58 % used, the exp unit
-// 38 %) and the round of waits between them and the MMAs (tensor pipe 36 %).  A chunk of 1001 tokens, 32 heads over 8 kv
+// Bound.  A step of two streams takes about 2300 cycles: the softmax warps' instructions (issue slots 60 % used, the exp unit
+// 40 %) and the round of waits between them and the MMAs (tensor pipe 39 %).  A chunk of 1001 tokens, 32 heads over 8 kv
 // heads of 128, 9001 positions: 187 us, 745 TFLOP/s, 16 us of it the joining kernel.  A unit's begin and end take 5000
 // cycles each, a launch 15000 before the first step, which is what few tokens cost.  With parts left out (of 195 us before
 // the last steps): 172 us without exponentials, 180 with an eighth of S's products, no less without the conversion of the codes.

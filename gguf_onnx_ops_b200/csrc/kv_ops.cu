@@ -77,13 +77,13 @@ cudaError_t run_rope(const RopeArgs& a, bool interleaved, cudaStream_t s) {
 // tile kernel costs 20 us in any case (two launches, a pipeline to fill).  Work is what the streaming kernel's line would
 // hold at most, from the page table's width and the window: lengths are on the device.
 // Streaming / tile in us, 8 kv heads, 16 sequences of 801 to 9001 tokens, and one of 65001:
-//   128 values: 16 rows 58 / 83, 55 / 72; 24 rows 99 / 84, 80 / 73; 48 rows 142 / 87, 108 / 74
-//   64 values: 16 rows 36 / 73, 33 / 60; 32 rows 61 / 73, 46 / 61; 48 rows 85 / 74, 60 / 61; 96 rows 159 / 76, 105 / 62
+//   128 values: 16 rows 60 / 79, 58 / 70; 24 rows 101 / 79, 86 / 71; 48 rows 144 / 82, 117 / 73
+//   64 values: 16 rows 36 / 68, 34 / 61; 32 rows 58 / 68, 47 / 61; 48 rows 81 / 68, 62 / 61; 96 rows 148 / 71, 106 / 62
 // and by work, in tiles of the line per SM:
-//   128 values: 128 rows, 3201 tokens (100) 28 / 27; 512 rows, 801 tokens (143) 30 / 36; 128 rows, 6401 tokens (187) 40 / 30;
-//   512 rows, 1601 tokens (230) 43 / 37
-//   64 values: 128 rows, 6401 tokens (187) 24 / 25; 512 rows, 1601 tokens (230) 27 / 31; 16 sequences, 128 rows, 201 tokens (311)
-//   31 / 17; 512 rows, 3201 tokens (400) 38 / 32
+//   128 values: 128 rows, 3201 tokens (100) 29 / 29; 512 rows, 801 tokens (143) 32 / 37; 128 rows, 6401 tokens (187) 41 / 32;
+//   512 rows, 1601 tokens (230) 44 / 38
+//   64 values: 128 rows, 6401 tokens (187) 25 / 26; 512 rows, 1601 tokens (230) 28 / 32; 16 sequences, 128 rows, 201 tokens (311)
+//   32 / 18; 512 rows, 3201 tokens (400) 39 / 34
 // 8 rows of 128 values taken as 16: 57 -> 84 us (one sequence of 131071 tokens).
 struct AttentionPlan {
   bool tile;
@@ -358,8 +358,9 @@ int gguf_draft_verify(const float* target, const float* draft_probs, const int32
   const bool wide = V % 4 == 0 && is_aligned(target, 16) && (!draft_probs || is_aligned(draft_probs, 16));
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  // A sequence's row is shared by as many CTAs (8 at most) as keep the whole call in one wave of two an SM.  131072 tokens, 8
-  // / 4 / 1 CTAs, in us: 16 sequences 8.5 / - / 26; 64 sequences 18.5 / 13.9 / 31.  32000 tokens, 256 sequences: 8 CTAs 47, one 13.5.
+  // A sequence's row is shared by as many CTAs (8 at most) as keep the whole call in one wave of two an SM.  8 / 4 / 2 / 1 CTAs, in
+  // us, rows from memory: 131072 tokens, 16 sequences 8.1 / 10.1 / 16.3 / 28.4, 64 sequences 21.1 / 17.9 / 22.6 / 35.5; 32000
+  // tokens, 256 sequences 50.2 / 26.0 / 18.7 / 15.7.  (64 sequences whose rows the L2 still holds: 17.5 / 13.3 / 17.2 / 31.5.)
   int ctas = kDraftCtas;
   while (ctas > 1 && B * ctas > 2 * sms) ctas /= 2;
   cudaLaunchConfig_t cfg = {};
